@@ -52,6 +52,14 @@ SYMBOLS = {
     "b2_copy_segments": (_int, [_vp, _vp, _vp, _i32, _vp]),
     "b2_images_to_u8": (_int, [_vp, _i32, _vp, _i64, _vp]),
     "b2_gate_residual": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "b2_quantize_mxfp4": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "b2_swiglu_quantize_mxfp4": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "b2_dequantize_mxfp4": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "b2_dequantize_int8_rowwise": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "b2_mxfp4_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp]),
+    "b2_mxfp4_linear": (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "b2_rmsnorm_residual_quant": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
+    "b2_rmsnorm_residual_mxfp4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
 }
 
 ABI_VERSION = 1

@@ -67,7 +67,7 @@ int b2_check_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "stream synchronize: %s", cudaGetErrorString(e));
   const unsigned int word = read_clear_status_gemm() | read_clear_status_gemm2() | read_clear_status_flash() |
-                            read_clear_status_flash2();
+                            read_clear_status_flash2() | read_clear_status_mxfp4();
   if (word == 0xffffffffu) return fail(B2_LAUNCH_FAILED, "status word could not be read");
   if (word != 0) return fail(B2_TIMEOUT, "device-side bounded wait gave up (code 0x%x)", word);
   return B2_OK;
@@ -345,6 +345,119 @@ int b2_flash_fwd(const void* q, const void* k, const void* v, void* out, int32_t
       return fail(B2_TOO_LARGE, "flash_fwd: stride too large");
   }
   return launch_flash_fwd(q, k, v, out, B, H, S, qs, ks, vs, scale, (cudaStream_t)stream);
+}
+
+static int check_mx_matrix(const char* who, const void* q, const void* scales, int64_t M, int64_t K) {
+  if (M < 0 || K < 0) return fail(B2_BAD_SHAPE, "%s: negative size M=%lld K=%lld", who, (long long)M, (long long)K);
+  if (K % 32 != 0) return fail(B2_NOT_WHITELISTED, "%s: K=%lld must be a multiple of 32 (the columns of one scale)", who, (long long)K);
+  if (M == 0 || K == 0) return B2_OK;
+  if (!q || !scales) return fail(B2_NULL_POINTER, "%s: null pointer", who);
+  if (!aligned16(q) || !aligned16(scales)) return fail(B2_BAD_STRIDE, "%s: elements and scales must be 16-byte aligned", who);
+  return -1;
+}
+
+int b2_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, void* stream) {
+  const int st = check_mx_matrix("quantize_mxfp4", q, scales, M, K);
+  if (st >= 0) return st;
+  B2_REQUIRE_PTR(x);
+  if (!aligned16(x)) return fail(B2_BAD_STRIDE, "quantize_mxfp4: x must be 16-byte aligned");
+  return launch_quantize_mxfp4(x, q, scales, M, K, false, (cudaStream_t)stream);
+}
+
+int b2_swiglu_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, void* stream) {
+  const int st = check_mx_matrix("swiglu_quantize_mxfp4", q, scales, M, K);
+  if (st >= 0) return st;
+  B2_REQUIRE_PTR(x);
+  if (!aligned16(x)) return fail(B2_BAD_STRIDE, "swiglu_quantize_mxfp4: x must be 16-byte aligned");
+  return launch_quantize_mxfp4(x, q, scales, M, K, true, (cudaStream_t)stream);
+}
+
+int b2_dequantize_mxfp4(const uint8_t* q, const uint8_t* scales, void* out, int64_t M, int64_t K, void* stream) {
+  const int st = check_mx_matrix("dequantize_mxfp4", q, scales, M, K);
+  if (st >= 0) return st;
+  B2_REQUIRE_PTR(out);
+  if (!aligned16(out)) return fail(B2_BAD_STRIDE, "dequantize_mxfp4: out must be 16-byte aligned");
+  return launch_dequantize_mxfp4(q, scales, out, M, K, (cudaStream_t)stream);
+}
+
+int b2_dequantize_int8_rowwise(const int8_t* q, const float* scale, void* out, int64_t M, int64_t K, void* stream) {
+  if (M < 0 || K < 0) return fail(B2_BAD_SHAPE, "dequantize_int8_rowwise: negative size M=%lld K=%lld", (long long)M, (long long)K);
+  if (M == 0 || K == 0) return B2_OK;
+  if (!q || !scale || !out) return fail(B2_NULL_POINTER, "dequantize_int8_rowwise: null pointer");
+  if ((reinterpret_cast<uintptr_t>(scale) & 3u) || (reinterpret_cast<uintptr_t>(out) & 1u))
+    return fail(B2_BAD_STRIDE, "dequantize_int8_rowwise: misaligned pointer");
+  return launch_dequantize_int8_rows(q, scale, out, M, K, (cudaStream_t)stream);
+}
+
+static int check_rmsnorm(const char* who, const void* x, const void* residual, const void* weight, const void* sum,
+                         const void* q, const void* scale, int64_t M, int64_t C, float eps) {
+  if (M < 0 || C <= 0) return fail(B2_BAD_SHAPE, "%s: bad size M=%lld C=%lld", who, (long long)M, (long long)C);
+  if (!(eps >= 0.0f) || std::isinf(eps)) return fail(B2_BAD_SHAPE, "%s: eps must be finite and >= 0", who);
+  if (M == 0) return B2_OK;
+  if (!x || !weight || !q || !scale) return fail(B2_NULL_POINTER, "%s: null pointer", who);
+  if ((residual == nullptr) != (sum == nullptr)) return fail(B2_NULL_POINTER, "%s: residual and sum come together", who);
+  if (sum != nullptr && (sum == x || sum == residual)) return fail(B2_BAD_STRIDE, "%s: sum must not alias an input", who);
+  if ((reinterpret_cast<uintptr_t>(x) & 1u) || (reinterpret_cast<uintptr_t>(residual) & 1u) ||
+      (reinterpret_cast<uintptr_t>(weight) & 1u) || (reinterpret_cast<uintptr_t>(sum) & 1u) ||
+      (reinterpret_cast<uintptr_t>(scale) & 3u))
+    return fail(B2_BAD_STRIDE, "%s: misaligned pointer", who);
+  return -1;
+}
+
+int b2_rmsnorm_residual_quant(const void* x, const void* residual, const void* weight, void* sum, int8_t* q,
+                              float* scale, int64_t M, int64_t C, float eps, void* stream) {
+  const int st = check_rmsnorm("rmsnorm_residual_quant", x, residual, weight, sum, q, scale, M, C, eps);
+  if (st >= 0) return st;
+  return launch_rmsnorm_residual(x, residual, weight, sum, q, scale, M, C, eps, false, (cudaStream_t)stream);
+}
+
+int b2_rmsnorm_residual_mxfp4(const void* x, const void* residual, const void* weight, void* sum, uint8_t* q,
+                              uint8_t* scales, int64_t M, int64_t C, float eps, void* stream) {
+  int st = check_rmsnorm("rmsnorm_residual_mxfp4", x, residual, weight, sum, q, scales, M, C, eps);
+  if (st >= 0) return st;
+  st = check_mx_matrix("rmsnorm_residual_mxfp4", q, scales, M, C);
+  if (st >= 0) return st;
+  if (C > 16384) return fail(B2_TOO_LARGE, "rmsnorm_residual_mxfp4: C=%lld exceeds 16384", (long long)C);
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(sum))
+    return fail(B2_BAD_STRIDE, "rmsnorm_residual_mxfp4: pointers must be 16-byte aligned");
+  return launch_rmsnorm_residual(x, residual, weight, sum, q, scales, M, C, eps, true, (cudaStream_t)stream);
+}
+
+static int check_mx_gemm(const char* who, const void* a, const void* a_scales, const void* w, const void* w_scales,
+                         const void* bias, int bias_kind, const void* out, int64_t M, int64_t N, int64_t K) {
+  if (bias_kind < B2_BIAS_NONE || bias_kind > B2_BIAS_FP32) return fail(B2_BAD_DTYPE, "%s: bias must be none, bfloat16, or float32", who);
+  if (M < 0 || N < 0 || K < 0) return fail(B2_BAD_SHAPE, "%s: negative size", who);
+  if (M == 0 || N == 0) return B2_OK;
+  if (K == 0) return fail(B2_BAD_SHAPE, "%s: K must be positive", who);
+  if (K % 32 != 0) return fail(B2_NOT_WHITELISTED, "%s: K=%lld must be a multiple of 32 (the columns of one scale)", who, (long long)K);
+  if (N % 8 != 0) return fail(B2_NOT_WHITELISTED, "%s: N=%lld must be a multiple of 8", who, (long long)N);
+  if (M > 0x7fffff00LL || N > 0x7fffff00LL || K > 0x7fffff00LL) return fail(B2_TOO_LARGE, "%s: dimension exceeds int32", who);
+  if (!a || !a_scales || !w || !w_scales || !out) return fail(B2_NULL_POINTER, "%s: null pointer", who);
+  if (bias_kind != B2_BIAS_NONE && !bias) return fail(B2_NULL_POINTER, "%s: bias kind %d with a null bias", who, bias_kind);
+  if (!aligned16(a) || !aligned16(a_scales) || !aligned16(w) || !aligned16(w_scales) || !aligned16(out))
+    return fail(B2_BAD_STRIDE, "%s: operands, scales and out must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(bias) & (bias_kind == B2_BIAS_FP32 ? 3u : 1u)) return fail(B2_BAD_STRIDE, "%s: misaligned bias", who);
+  return -1;
+}
+
+int b2_mxfp4_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
+                  const void* bias, int bias_kind, void* out, int64_t M, int64_t N, int64_t K, void* stream) {
+  const int st = check_mx_gemm("mxfp4_gemm", a, a_scales, w, w_scales, bias, bias_kind, out, M, N, K);
+  if (st >= 0) return st;
+  return launch_mxfp4_gemm(a, a_scales, w, w_scales, bias, bias_kind, out, M, N, K, (cudaStream_t)stream);
+}
+
+int b2_mxfp4_linear(const void* x, int input_act, const uint8_t* w, const uint8_t* w_scales, const void* bias,
+                    int bias_kind, void* out, uint8_t* q_scratch, uint8_t* s_scratch, int64_t M, int64_t N,
+                    int64_t K, void* stream) {
+  if (input_act != B2_ACT_NONE && input_act != B2_ACT_SWIGLU) return fail(B2_BAD_DTYPE, "mxfp4_linear: unknown input activation %d", input_act);
+  int st = check_mx_gemm("mxfp4_linear", q_scratch, s_scratch, w, w_scales, bias, bias_kind, out, M, N, K);
+  if (st >= 0) return st;
+  B2_REQUIRE_PTR(x);
+  if (!aligned16(x)) return fail(B2_BAD_STRIDE, "mxfp4_linear: x must be 16-byte aligned");
+  st = launch_quantize_mxfp4(x, q_scratch, s_scratch, M, K, input_act == B2_ACT_SWIGLU, (cudaStream_t)stream);
+  if (st != B2_OK) return st;
+  return launch_mxfp4_gemm(q_scratch, s_scratch, w, w_scales, bias, bias_kind, out, M, N, K, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -59,11 +59,26 @@ int launch_flash_fwd_pair(const void* q, const void* k, const void* v, void* out
                           const int64_t* qs, const int64_t* ks, const int64_t* vs, float scale,
                           cudaStream_t stream);
 
+// MXFP4 (mxfp4.cuh).  swiglu: x is [M, 2K], gate columns then up columns
+int launch_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, bool swiglu,
+                          cudaStream_t stream);
+int launch_dequantize_mxfp4(const uint8_t* q, const uint8_t* scales, void* out, int64_t M, int64_t K,
+                            cudaStream_t stream);
+int launch_dequantize_int8_rows(const int8_t* q, const float* scale, void* out, int64_t M, int64_t K,
+                                cudaStream_t stream);
+int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale,
+                      const void* bias, int bias_kind, void* out, int64_t M, int64_t N, int64_t K,
+                      cudaStream_t stream);
+// residual == nullptr: the norm of x alone, `sum` untouched.  mx: MXFP4 output, otherwise int8 rows
+int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* sum, void* q, void* scale,
+                            int64_t M, int64_t C, float eps, bool mx, cudaStream_t stream);
+
 int launch_bounded_wait_selftest(cudaStream_t stream);
 // Read and clear the device-side status word of a tensor-core translation unit.
 unsigned int read_clear_status_gemm();
 unsigned int read_clear_status_gemm2();
 unsigned int read_clear_status_flash();
 unsigned int read_clear_status_flash2();
+unsigned int read_clear_status_mxfp4();
 
 }  // namespace b2

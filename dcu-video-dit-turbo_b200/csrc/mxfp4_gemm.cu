@@ -1,0 +1,386 @@
+// Product of two MXFP4 matrices: out bf16 [M, N] = bf16(A [M, K] . W [N, K]^T + bias), fp32
+// accumulation, one rounding.
+//
+// tcgen05.mma kind::mxf4 multiplies packed 4-bit operands (64 columns per instruction) and applies
+// the two power-of-two scales of every 32 columns inside the tensor core, so neither operand is
+// ever expanded.  Elements go from global memory to shared memory by TMA (128-byte swizzle, 256
+// columns per stage); the scale tiles, already in tensor-memory order (mxfp4.cuh), by plain bulk
+// copies, and from there into tensor memory by tcgen05.cp.
+//
+//   warp 0     loads: per stage A, W, A's scales, W's scales
+//   warp 1     one lane copies a stage's scales into tensor memory and issues its MMAs
+//   warps 2-5  epilogue: accumulators -> bias -> bf16 -> staging tile -> TMA store
+//
+// Tensor memory (512 columns): a tile's 256 accumulator columns, twice, leave no room for scales,
+// so the two accumulators overlap by 64 columns (0-255 and 192-447) and the scales have the last
+// 64, two stages of 24.  The epilogue reads the shared 64 columns first and then lets the next
+// tile's MMAs begin, so the main loop stands still for two tensor-memory loads per tile and not for
+// a whole epilogue.  A stage's scales may replace those of two stages before only when that stage's
+// MMAs are complete (their commit is waited for): the order of an MMA and a later copy into its
+// scales is not promised.
+// Every wait is bounded; on a timeout the kernel records a status word and returns.
+#include "b2_common.cuh"
+#include "b2_launch.h"
+#include "gemm_epilogue.cuh"
+#include "mxfp4.cuh"
+#include "sm100_ptx.cuh"
+
+namespace b2 {
+
+unsigned int read_clear_status_mxfp4() { return read_and_clear_device_status(); }
+
+namespace {
+
+constexpr int BM = 128;                    // rows per CTA
+constexpr int BN = 256;                    // columns per tile
+constexpr int BKE = 256;                   // columns of K per stage
+constexpr int BKB = BKE / 2;               // ... in bytes: one 128-byte swizzled line
+constexpr int UMMA_K = 64;
+constexpr int NUM_THREADS = 192;
+constexpr int EPI_THREADS = 128;
+constexpr int TMEM_COLS = 512;
+constexpr int ACC1 = 192;                  // first column of the second accumulator
+constexpr int SHARED_COLS = 64;            // columns the two accumulators have in common
+constexpr int SF_COL = 448;                // scales: two buffers of 32 columns
+constexpr int SF_STRIDE = 32;
+constexpr int SFB_COL = 8;                 // within a buffer: A's 2 x 4 columns, then W's 2 x 8
+
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BKB;          // 16 KB
+constexpr int B_BYTES = BN * BKB;          // 32 KB
+constexpr int SFA_BYTES = 2 * kMxTileBytes;
+constexpr int SFB_BYTES = 4 * kMxTileBytes;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SMEM_SF = STAGES * STAGE_BYTES;
+constexpr int SF_STAGE = SFA_BYTES + SFB_BYTES;
+constexpr int SMEM_OUT = SMEM_SF + STAGES * SF_STAGE;
+constexpr int SMEM_BIAS = SMEM_OUT + (EPI_THREADS / 32) * kEpiStageBytes;
+constexpr int SMEM_BARS = SMEM_BIAS + 2 * BN * 4;
+constexpr int NUM_BARS = 2 * STAGES + 2 + 1 + 2;
+constexpr int SMEM_TOTAL = 1024 + SMEM_BARS + NUM_BARS * 8 + 16;
+static_assert(SMEM_TOTAL <= 227 * 1024, "shared memory budget");
+static_assert(SMEM_OUT % 1024 == 0, "staging tiles are 1024-byte aligned");
+
+struct MxGemmArgs {
+  int M, N, K;
+  int tiles_m, tiles_n, num_tiles, k_blocks, group_m;
+  int k_tiles;                 // scale tiles along K
+  int b_row_tiles;             // scale tiles along W's rows
+  const uint8_t* a_scale;
+  const uint8_t* w_scale;
+  const void* bias;
+  int bias_kind;
+};
+
+__device__ __forceinline__ void decode_tile(int tile, const MxGemmArgs& a, int& m_idx, int& n_idx) {
+  const int per_group = a.group_m * a.tiles_n;
+  const int group = tile / per_group;
+  const int first_m = group * a.group_m;
+  const int rows = min(a.group_m, a.tiles_m - first_m);
+  const int in_group = tile - group * per_group;
+  m_idx = first_m + in_group % rows;
+  n_idx = in_group / rows;
+}
+
+// contiguous global -> shared copy counted on a barrier; addresses and size multiples of 16
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// one scale tile: 32 lines of 16 bytes -> 32 lanes x 4 columns, repeated in all four lane quarters
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
+  // no swizzle; 8 lines of 16 bytes are contiguous, the next 8 follow 128 bytes on
+  const uint64_t desc = (uint64_t)((smem_addr >> 4) & 0x3fffu) | (1ull << 16) | (8ull << 32) | (1ull << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor of kind::mxf4: scale word halves 4-5 (W) and 29-30 (A), formats 7-9 and
+// 10-11 (1 = E2M1), N >> 3 in 17-22, scale format bit 23 (1 = E8M0), M >> 4 from bit 24.
+__host__ __device__ constexpr uint32_t mx_idesc(uint32_t m, uint32_t n, uint32_t half) {
+  return ((half * 2) << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | ((half * 2) << 29);
+}
+
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                  const __grid_constant__ CUtensorMap tmap_out, const MxGemmArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* bias_s = reinterpret_cast<float*>(smem + SMEM_BIAS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + STAGES * 8;
+  const uint32_t tfull0 = empty0 + STAGES * 8;   // accumulator complete (2)
+  const uint32_t tfree = tfull0 + 2 * 8;         // the shared columns of the tile before are read
+  const uint32_t sfree0 = tfree + 8;             // MMAs that read scale buffer 0 / 1 are complete
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + s * 8, 1);
+      mbar_init(empty0 + s * 8, 1);
+    }
+    mbar_init(tfull0, 1);
+    mbar_init(tfull0 + 8, 1);
+    mbar_init(tfree, EPI_THREADS / 32);
+    mbar_init(sfree0, 1);
+    mbar_init(sfree0 + 8, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_out);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+        int m_idx, n_idx;
+        decode_tile(tile, args, m_idx, n_idx);
+        const uint8_t* sfa = args.a_scale + (int64_t)m_idx * args.k_tiles * kMxTileBytes;
+        const uint8_t* sfb = args.w_scale + (int64_t)n_idx * 2 * args.k_tiles * kMxTileBytes;
+        const int b_tiles = min(2, args.b_row_tiles - n_idx * 2);
+        for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (!(ok = mbar_wait(empty0 + stage * 8, phase ^ 1, abort_flag, kStatusGemmTimeout))) break;
+          const uint32_t bar = full0 + stage * 8;
+          const uint32_t dst = ring + stage * STAGE_BYTES;
+          const uint32_t sf = ring + SMEM_SF + stage * SF_STAGE;
+          // the last stage may hold one scale tile per row tile only
+          const uint32_t sf_bytes = (uint32_t)min(2, args.k_tiles - 2 * kb) * kMxTileBytes;
+          mbar_expect_tx(bar, STAGE_BYTES + (1 + b_tiles) * sf_bytes);
+          tma_load_2d(dst, &tmap_a, bar, kb * BKB, m_idx * BM);
+          tma_load_2d(dst + A_BYTES, &tmap_b, bar, kb * BKB, n_idx * BN);
+          bulk_load(sf, sfa + (int64_t)kb * 2 * kMxTileBytes, sf_bytes, bar);
+          for (int t = 0; t < b_tiles; ++t)
+            bulk_load(sf + SFA_BYTES + t * 2 * kMxTileBytes,
+                      sfb + ((int64_t)t * args.k_tiles + kb * 2) * kMxTileBytes, sf_bytes, bar);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int sbuf = 0;
+      uint32_t sphase = 0;
+      int buf = 0;
+      uint32_t fphase = 0;
+      bool first = true, ok = true;
+      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+        // the tile before must have left the columns that this one's accumulator shares with it
+        if (!first) {
+          if (!(ok = mbar_wait(tfree, fphase, abort_flag, kStatusGemmTimeout))) break;
+          fphase ^= 1;
+          tc_fence_after();
+        }
+        first = false;
+        const uint32_t d_tmem = tmem_base + (buf ? ACC1 : 0);
+        for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (!(ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout))) break;
+          if (!(ok = mbar_wait(sfree0 + sbuf * 8, sphase ^ 1, abort_flag, kStatusGemmTimeout))) break;
+          tc_fence_after();
+          const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
+          const uint32_t sf = ring + SMEM_SF + stage * SF_STAGE;
+          const uint32_t sf_tmem = tmem_base + SF_COL + sbuf * SF_STRIDE;
+          // [k tile][row group of 32]: 4 columns of A per k tile, 8 of W
+          for (int kt = 0; kt * 2 < steps; ++kt) {
+            scales_to_tmem(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
+            for (int t = 0; t < 2; ++t)
+              scales_to_tmem(sf_tmem + SFB_COL + kt * 8 + t * 4, sf + SFA_BYTES + (t * 2 + kt) * kMxTileBytes);
+          }
+          const uint32_t a_addr = ring + stage * STAGE_BYTES;
+          const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
+          const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
+          for (int k = 0; k < steps; ++k)
+            mma_mxf4(d_tmem, adesc + 2 * k, bdesc + 2 * k, (k & 1) ? mx_idesc(BM, BN, 1) : mx_idesc(BM, BN, 0),
+                     sf_tmem + (k >> 1) * 4, sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
+          tc_commit(sfree0 + sbuf * 8);
+          tc_commit(empty0 + stage * 8);
+          sbuf ^= 1;
+          if (sbuf == 0) sphase ^= 1;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit(tfull0 + buf * 8);
+        buf ^= 1;
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - 64;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    const uint32_t stage = ring + SMEM_OUT + quarter * kEpiStageBytes;
+    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
+      int m_idx, n_idx;
+      decode_tile(tile, args, m_idx, n_idx);
+      const int col0 = n_idx * BN;
+      const int row_warp = m_idx * BM + quarter * 32;
+      float* bias = bias_s + buf * BN;
+      for (int c = et; c < BN; c += EPI_THREADS) {
+        float b = 0.f;
+        if (col0 + c < args.N) {
+          if (args.bias_kind == B2_BIAS_BF16) b = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(args.bias)[col0 + c]);
+          if (args.bias_kind == B2_BIAS_FP32) b = reinterpret_cast<const float*>(args.bias)[col0 + c];
+        }
+        bias[c] = b;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (!mbar_wait(tfull0 + buf * 8, buf_phase, abort_flag, kStatusGemmTimeout)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (buf ? ACC1 : 0) + ((uint32_t)(quarter * 32) << 16);
+      // the columns shared with the other accumulator come first: the last 64 of the first one,
+      // the first 64 of the second
+#pragma unroll 1
+      for (int i = 0; i < BN / 64; ++i) {
+        const int c = buf ? 64 * i : (64 * i + BN - SHARED_COLS) % BN;
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(taddr + c, v[0]);
+        tmem_ld_32x32b_x32(taddr + c + 32, v[1]);
+        tmem_wait_ld();
+        if (i == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tfree);
+        }
+        if (col0 + c >= args.N) continue;
+        if (lane == 0) bulk_wait_group_read<0>();   // the previous store has read the tile
+        __syncwarp();
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t o[16];
+          const float* bc = bias + c + 32 * hh;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            o[j] = pack_bf16x2_rn(__uint_as_float(v[hh][2 * j]) + bc[2 * j], __uint_as_float(v[hh][2 * j + 1]) + bc[2 * j + 1]);
+          epilogue_stage_write(stage, lane, hh, o);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && row_warp < args.M) {
+          tma_store_2d(&tmap_out, stage, col0 + c, row_warp);
+          bulk_commit_group();
+        }
+      }
+      buf ^= 1;
+      if (buf == 0) buf_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_group<0>();   // this warp's stores are complete before the CTA may retire
+  }
+
+  __syncwarp();
+  if (*abort_flag != 0) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 200000) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+int encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int box_rows) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
+  const cuuint32_t box[2] = {BKB, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: tensor map encode failed (%d)", (int)r);
+  return B2_OK;
+}
+
+int encode_out(CUtensorMap* map, void* base, int64_t M, int64_t N) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+  const cuuint64_t strides[1] = {(cuuint64_t)N * 2};
+  const cuuint32_t box[2] = {64, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: output tensor map encode failed (%d)", (int)r);
+  return B2_OK;
+}
+
+}  // namespace
+
+int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale,
+                      const void* bias, int bias_kind, void* out, int64_t M, int64_t N, int64_t K,
+                      cudaStream_t stream) {
+  static PerDeviceSetup per_device;
+  const DeviceSlot* slot = nullptr;
+  const int setup_status = per_device.get("mxfp4_gemm", [](int dev, DeviceSlot& s) -> int {
+    cudaError_t e = cudaFuncSetAttribute(mxfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL);
+    if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
+    s.a = kNumSMsB200;
+    cudaDeviceGetAttribute(&s.a, cudaDevAttrMultiProcessorCount, dev);
+    return B2_OK;
+  }, &slot);
+  if (setup_status != B2_OK) return setup_status;
+  CUtensorMap ta, tb, tout;
+  int st = encode_operand(&ta, A, M, K, BM);
+  if (st != B2_OK) return st;
+  st = encode_operand(&tb, W, N, K, BN);
+  if (st != B2_OK) return st;
+  st = encode_out(&tout, out, M, N);
+  if (st != B2_OK) return st;
+  MxGemmArgs a;
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.tiles_m = (int)((M + BM - 1) / BM);
+  a.tiles_n = (int)((N + BN - 1) / BN);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  if (tiles > 0x7fffffffLL) return fail(B2_TOO_LARGE, "mxfp4_gemm: too many tiles");
+  a.num_tiles = (int)tiles;
+  a.k_blocks = (int)((K + BKE - 1) / BKE);
+  a.group_m = 16;
+  a.k_tiles = (int)((K + kMxTileCols - 1) / kMxTileCols);
+  a.b_row_tiles = (int)((N + kMxTileRows - 1) / kMxTileRows);
+  a.a_scale = a_scale;
+  a.w_scale = w_scale;
+  a.bias = bias;
+  a.bias_kind = bias_kind;
+  const int grid = a.num_tiles < slot->a ? a.num_tiles : slot->a;
+  mxfp4_gemm_kernel<<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(ta, tb, tout, a);
+  return check_launch("mxfp4_gemm");
+}
+
+}  // namespace b2

@@ -1,0 +1,247 @@
+// RMSNorm with the residual's addition and a quantised output: the producer of a quantised linear.
+//
+//   s = bf16(x + residual)                      (stored: the residual stream of the next layer)
+//   y = s / sqrt(mean(s^2) + eps) * weight      (fp32)
+//   int8    scale = max|y| / 127 per row, at least 1e-30;  q = round half even(y / scale)
+//   mxfp4   per block of 32 columns (mxfp4.cuh)
+//
+// Bound by memory: 4 bytes in and 2 + 1 (2 + 17/32) bytes out per element.  A row is held by TPR
+// threads in registers from its only read to its quantised write; y is never rounded to bf16 in
+// between.  A thread keeps the same columns of every row, so the weight is read once per CTA.
+// The int8 scale divides by the fp32 scale that is stored, so q * scale is within half a step of y.
+#include "b2_common.cuh"
+#include "b2_launch.h"
+#include "mxfp4.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RmsArgs {
+  const uint4* x;
+  const uint4* residual;   // null: s = x and nothing is stored to `sum`
+  const uint4* weight;
+  uint4* sum;
+  void* q;                 // int8 [M, C] or packed [M, C/2]
+  void* scale;             // fp32 [M] or scale tiles
+  int64_t M;
+  int cvec;                // C / 8
+  float inv_c, eps;
+};
+
+// What a row's int8 scale and multiplier are, from the row's largest magnitude.  Rows with a NaN or
+// an infinity keep that in the scale and get zero elements.
+__device__ __forceinline__ float int8_scale(float absmax, float& inv, bool& zero_row) {
+  float s = absmax != absmax ? absmax : fmaxf(__fmul_rn(absmax, kInv127), 1.0e-30f);
+  zero_row = !(s <= 3.4028234e38f);
+  inv = __frcp_rn(s);
+  return s;
+}
+// Round half even of a value within +-127 (a few units in the last place over): low byte of the sum.
+__device__ __forceinline__ uint32_t int8_bits(float v) { return __float_as_uint(v + 12582912.0f) & 0xffu; }
+
+template <int TPR, int VPT, bool MX>
+__global__ void __launch_bounds__(kThreads)
+rmsnorm_residual_kernel(const RmsArgs a) {
+  __shared__ float red[2][kThreads / 32];
+  constexpr int RPC = kThreads / TPR;
+  const int slot = threadIdx.x / TPR;
+  const int lane = threadIdx.x % TPR;
+  uint4 wt[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = lane + i * TPR;
+    wt[i] = c < a.cvec ? __ldg(a.weight + c) : make_uint4(0, 0, 0, 0);
+  }
+  // 4-bit scales come in tiles of 128 rows: the rows that fill the last tile are walked too
+  const int64_t rows = MX ? (a.M + kMxTileRows - 1) / kMxTileRows * kMxTileRows : a.M;
+  const int col_tiles = (a.cvec + 15) / 16;
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * RPC; row0 < rows; row0 += (int64_t)gridDim.x * RPC) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.M;
+    uint4 v[VPT], r[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = lane + i * TPR;
+      const bool in = live && c < a.cvec;
+      v[i] = in ? ldg_stream(a.x + row * a.cvec + c) : make_uint4(0, 0, 0, 0);
+      r[i] = in && a.residual != nullptr ? ldg_stream(a.residual + row * a.cvec + c) : make_uint4(0, 0, 0, 0);
+    }
+    uint64_t ss2[2] = {0ull, 0ull};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = lane + i * TPR;
+      uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      if (a.residual != nullptr) {
+        const uint32_t rw[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = bf16x2_add_rn(w[j], rw[j]);
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (live && c < a.cvec) a.sum[row * a.cvec + c] = v[i];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t e = bf16x2_to_f32x2(w[j]);
+        ss2[j & 1] = fma2(e, e, ss2[j & 1]);
+      }
+    }
+    float a0, a1, b0, b1;
+    unpack2(ss2[0], a0, a1);
+    unpack2(ss2[1], b0, b1);
+    // consecutive reductions use the two buffers in turn
+    const float ss = slot_allreduce<kThreads, TPR>((a0 + a1) + (b0 + b1), red[turn], slot, SumOp());
+    turn ^= 1;
+    const float rstd = rsqrtf(ss * a.inv_c + a.eps);
+    const uint64_t rstd2 = pack2(rstd, rstd);
+    float y[VPT][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      const uint32_t ww[4] = {wt[i].x, wt[i].y, wt[i].z, wt[i].w};
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unpack2(mul2(mul2(bf16x2_to_f32x2(w[j]), rstd2), bf16x2_to_f32x2(ww[j])), y[i][2 * j], y[i][2 * j + 1]);
+        m = max(m, max(__float_as_uint(y[i][2 * j]) & 0x7fffffffu, __float_as_uint(y[i][2 * j + 1]) & 0x7fffffffu));
+      }
+      if constexpr (MX) {
+        const int c = lane + i * TPR;
+        // columns outside the row (and rows outside the matrix) are zeros times rstd: not NaN unless
+        // rstd is one, so they are cleared
+        if (!live || c >= a.cvec) m = 0;
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t byte = mx_scale_byte(m >> 23);
+        const float inv = mx_inverse_scale(byte);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[i][j] *= inv;
+        const uint32_t word = mx_gather_word(byte, 0xffffffffu);
+        if (live && c < a.cvec)
+          reinterpret_cast<uint32_t*>(a.q)[row * a.cvec + c] = byte == 255u ? 0u : mx_pack8(y[i]);
+        if ((c & 15) == 0 && c < col_tiles * 16)
+          *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.scale) +
+                                       ((row / kMxTileRows) * col_tiles + c / 16) * kMxTileBytes +
+                                       mx_scale_offset((int)(row % kMxTileRows), 0)) = word;
+      } else {
+        most = max(most, m);
+      }
+    }
+    if constexpr (!MX) {
+      // the weight's vector of a column outside the row is zero: such columns add nothing to the
+      // maximum, but for a NaN that the row's own columns have as well
+      const float absmax = slot_allreduce<kThreads, TPR>(__uint_as_float(most), red[turn], slot, NanMaxOp());
+      turn ^= 1;
+      float inv;
+      bool zero_row;
+      const float s = int8_scale(absmax, inv, zero_row);
+      if (live) {
+        if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = s;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = lane + i * TPR;
+          if (c < a.cvec) {
+            uint2 o = make_uint2(0, 0);
+            if (!zero_row) {
+              uint32_t b[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) b[j] = int8_bits(y[i][j] * inv);
+              o.x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
+              o.y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
+            }
+            reinterpret_cast<uint2*>(a.q)[row * a.cvec + c] = o;
+          }
+        }
+      }
+    }
+  }
+}
+
+// int8 form for any width and alignment: one CTA per row, which is read three times (the second and
+// third time from L2).
+__global__ void __launch_bounds__(kThreads)
+rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ residual,
+                                      const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ sum,
+                                      int8_t* __restrict__ q, float* __restrict__ scale, int64_t M, int64_t C,
+                                      float inv_c, float eps) {
+  __shared__ float red[2][kThreads / 32];
+  for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
+    const int64_t at = row * C;
+    auto value = [&](int64_t c) {
+      const __nv_bfloat16 v = x[at + c];
+      return residual != nullptr ? __bfloat162float(__hadd_rn(v, residual[at + c])) : __bfloat162float(v);
+    };
+    float ss = 0.f;
+    for (int64_t c = threadIdx.x; c < C; c += kThreads) {
+      const float v = value(c);
+      if (residual != nullptr) sum[at + c] = __float2bfloat16_rn(v);
+      ss = fmaf(v, v, ss);
+    }
+    ss = slot_allreduce<kThreads, kThreads>(ss, red[0], 0, SumOp());
+    const float rstd = rsqrtf(ss * inv_c + eps);
+    uint32_t most = 0;
+    for (int64_t c = threadIdx.x; c < C; c += kThreads)
+      most = max(most, __float_as_uint(value(c) * rstd * __bfloat162float(weight[c])) & 0x7fffffffu);
+    const float absmax = slot_allreduce<kThreads, kThreads>(__uint_as_float(most), red[1], 0, NanMaxOp());
+    float inv;
+    bool zero_row;
+    const float s = int8_scale(absmax, inv, zero_row);
+    if (threadIdx.x == 0) scale[row] = s;
+    for (int64_t c = threadIdx.x; c < C; c += kThreads)
+      q[at + c] = zero_row ? (int8_t)0 : (int8_t)int8_bits(value(c) * rstd * __bfloat162float(weight[c]) * inv);
+  }
+}
+
+}  // namespace
+
+int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* sum, void* q, void* scale,
+                            int64_t M, int64_t C, float eps, bool mx, cudaStream_t stream) {
+  const float inv_c = (float)(1.0 / (double)C);
+  const bool vector = C % 8 == 0 && C <= 16384 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
+                      aligned16(sum) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  if (!vector) {
+    if (mx) return fail(B2_NOT_WHITELISTED, "rmsnorm_residual_mxfp4: C=%lld exceeds 16384", (long long)C);
+    const int64_t cap = (int64_t)kNumSMsB200 * 8;
+    rmsnorm_residual_quant_generic_kernel<<<(unsigned)(M < cap ? M : cap), kThreads, 0, stream>>>(
+        (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)weight, (__nv_bfloat16*)sum,
+        (int8_t*)q, (float*)scale, M, C, inv_c, eps);
+    return check_launch("rmsnorm_residual_quant");
+  }
+  RmsArgs a;
+  a.x = (const uint4*)x;
+  a.residual = (const uint4*)residual;
+  a.weight = (const uint4*)weight;
+  a.sum = (uint4*)sum;
+  a.q = q;
+  a.scale = scale;
+  a.M = M;
+  a.cvec = (int)(C / 8);
+  a.inv_c = inv_c;
+  a.eps = eps;
+  const int64_t rows = mx ? (M + kMxTileRows - 1) / kMxTileRows * kMxTileRows : M;
+#define B2_RMS(TPR, VPT)                                                                     \
+  do {                                                                                       \
+    const int64_t need = (rows + kThreads / TPR - 1) / (kThreads / TPR);                     \
+    const int64_t cap = (int64_t)kNumSMsB200 * 8;                                            \
+    const unsigned g = (unsigned)(need < cap ? need : cap);                                  \
+    if (mx)                                                                                  \
+      rmsnorm_residual_kernel<TPR, VPT, true><<<g, kThreads, 0, stream>>>(a);                \
+    else                                                                                     \
+      rmsnorm_residual_kernel<TPR, VPT, false><<<g, kThreads, 0, stream>>>(a);               \
+  } while (0)
+  // the fewest threads that hold a row at four vectors each (three where that fits exactly)
+  if (C <= 256) B2_RMS(32, 1);
+  else if (C <= 1024) B2_RMS(32, 4);
+  else if (C <= 2048) B2_RMS(64, 4);
+  else if (C <= 3072) B2_RMS(128, 3);
+  else if (C <= 4096) B2_RMS(128, 4);
+  else if (C <= 6144) B2_RMS(256, 3);
+  else if (C <= 8192) B2_RMS(256, 4);
+  else B2_RMS(256, 8);
+#undef B2_RMS
+  return check_launch("rmsnorm_residual");
+}
+
+}  // namespace b2

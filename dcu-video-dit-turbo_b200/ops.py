@@ -584,6 +584,174 @@ def gate_residual_(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor) -> torc
     return x
 
 
+# ---- MXFP4 (no counterpart in the reference) -------------------------------------
+
+MX_BLOCK = 32    # columns that share a scale
+
+
+def mxfp4_scale_shape(rows: int, columns: int) -> tuple[int, int, int]:
+    """Shape of the scale bytes of a [rows, columns] matrix: tiles of 128 rows x 4 blocks of 32
+    columns, in which the byte of row r and block b is (r % 32) * 16 + (r // 32) * 4 + b."""
+    return (-(-rows // 128), -(-columns // 128), 512)
+
+
+def _mx_empty(rows: int, columns: int, device):
+    return (torch.empty((rows, columns // 2), dtype=torch.uint8, device=device),
+            torch.empty(mxfp4_scale_shape(rows, columns), dtype=torch.uint8, device=device))
+
+
+def _require_mx(q: torch.Tensor, s: torch.Tensor, what: str) -> tuple[int, int]:
+    """Checks a quantised matrix (elements, scales); returns its rows and columns."""
+    _require(q.is_cuda and s.is_cuda and s.device == q.device, f"{what} and its scales must be on the same CUDA device")
+    _require(q.dtype == torch.uint8 and s.dtype == torch.uint8, f"{what} and its scales must be uint8")
+    _require(q.dim() == 2 and q.is_contiguous() and s.is_contiguous(), f"{what} must be a contiguous [M, K/2] tensor with contiguous scales")
+    m, k = q.shape[0], 2 * q.shape[1]
+    _require(k % MX_BLOCK == 0, f"{what} must have a multiple of {MX_BLOCK} columns")
+    _require(tuple(s.shape) == mxfp4_scale_shape(m, k),
+             f"the scales of {what} must have shape {mxfp4_scale_shape(m, k)}, got {tuple(s.shape)}")
+    return m, k
+
+
+def _quantize_mxfp4(name: str, x: torch.Tensor, halves: int):
+    _require(x.is_cuda, "input must be on the CUDA device")
+    _require(x.is_contiguous(), "input must be contiguous")
+    _require(x.dtype == torch.bfloat16, "input must be bfloat16")
+    _require(x.dim() == 2, "input must be a two-dimensional tensor")
+    m, k = x.shape[0], x.shape[1] // halves
+    _require(x.shape[1] % (halves * MX_BLOCK) == 0, f"input width must be a multiple of {halves * MX_BLOCK}")
+    q, s = _mx_empty(m, k, x.device)
+    if m and k:
+        _call(name, x, x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, _stream(x),
+              work=("hbm", 2 * halves * m * k + m * k // 2 + m * k // MX_BLOCK))
+    return [q, s]
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """bf16 [M,K] -> [uint8 [M,K/2], uint8 scales]: microscaled 4-bit floating point, a power-of-two
+    scale 2^(floor(log2(max|x|)) - 2) per 32 columns, elements +-{0, .5, 1, 1.5, 2, 3, 4, 6} to the
+    nearest with ties to the even code, two per byte (even column in the low half).  The scales'
+    layout is `mxfp4_scale_shape`'s, the one `mxfp4_gemm` reads."""
+    return _quantize_mxfp4("b2_quantize_mxfp4", x, 1)
+
+
+def swiglu_quantize_mxfp4(x: torch.Tensor):
+    """bf16 [M,2K] -> [uint8 [M,K/2], uint8 scales]: silu(gate)*up in fp32, then the quantiser."""
+    return _quantize_mxfp4("b2_swiglu_quantize_mxfp4", x, 2)
+
+
+def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    """bf16 [M,K]: the values of a quantised matrix."""
+    m, k = _require_mx(q, s, "the matrix")
+    out = torch.empty((m, k), dtype=torch.bfloat16, device=q.device)
+    if m and k:
+        _call("b2_dequantize_mxfp4", q, q.data_ptr(), s.data_ptr(), out.data_ptr(), m, k, _stream(q),
+              work=("hbm", 2 * m * k + m * k // 2 + m * k // MX_BLOCK))
+    return out
+
+
+def dequantize_int8_rowwise(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """bf16 [M,K] = q * scale[row]: the values of rowwise int8 (scale fp32, M values)."""
+    _require(q.is_cuda and q.dtype == torch.int8 and q.dim() == 2 and q.is_contiguous(),
+             "q must be a contiguous CUDA int8 [M,K] tensor")
+    _require_vector(scale, q, q.shape[0], torch.float32, "scale")
+    m, k = q.shape
+    out = torch.empty((m, k), dtype=torch.bfloat16, device=q.device)
+    if m and k:
+        _call("b2_dequantize_int8_rowwise", q, q.data_ptr(), scale.data_ptr(), out.data_ptr(), m, k, _stream(q),
+              work=("hbm", 3 * m * k + 4 * m))
+    return out
+
+
+def mxfp4_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               bias: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [M,N] = a @ w.T + bias of two quantised matrices (a [M,K], w [N,K], bias bf16 or fp32
+    [N]): the 4-bit operands and their scales go to the tensor core as they are; fp32 sums, one
+    rounding.  N must be a multiple of 8."""
+    m, k = _require_mx(a, a_scale, "a")
+    n, kw = _require_mx(w, w_scale, "w")
+    _require(w.device == a.device, "all inputs must be on the same device")
+    _require(k == kw, "shape mismatch")
+    _require(n % 8 == 0, "the output width must be a multiple of 8")
+    _require(k > 0, "the inner dimension must be positive")
+    kind = _bias_kind(bias, n, a.device)
+    out = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+    if m and n:
+        _call("b2_mxfp4_gemm", a, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+              _ptr(bias) if kind else None, kind, out.data_ptr(), m, n, k, _stream(a), work=("mxfp4", 2 * m * n * k))
+    return out
+
+
+def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                 input_act: str | None = None) -> torch.Tensor:
+    """One C call for (activation) -> quantize -> product.  x bf16 [M,K] (or [M,2K] with
+    input_act="swiglu"); w, w_scale a quantised [N,K] weight."""
+    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(),
+             "x must be a contiguous CUDA bf16 [M,K] tensor")
+    n, k = _require_mx(w, w_scale, "w")
+    act = {None: ACT_NONE, "swiglu": ACT_SWIGLU}.get(input_act, -1)
+    _require(act >= 0, f"unknown input activation {input_act!r}")
+    _require(w.device == x.device, "all inputs must be on the same device")
+    width = 2 * k if act == ACT_SWIGLU else k
+    if x.shape[1] != width:
+        raise ValueError(f"Input and weight inner dimensions must match, got {x.shape[1]} and {width}")
+    _require(n % 8 == 0, "the output width must be a multiple of 8")
+    _require(k > 0, "the inner dimension must be positive")
+    m = x.shape[0]
+    kind = _bias_kind(bias, n, x.device)
+    out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    if m and n:
+        qs, ss = _mx_empty(m, k, x.device)
+        _call("b2_mxfp4_linear", x, x.data_ptr(), act, w.data_ptr(), w_scale.data_ptr(), _ptr(bias) if kind else None,
+              kind, out.data_ptr(), qs.data_ptr(), ss.data_ptr(), m, n, k, _stream(x), launches=2,
+              work=("mxfp4", 2 * m * n * k))
+    return out
+
+
+# ---- RMSNorm with the residual's addition (no counterpart in the reference) ---------
+
+def _rmsnorm_inputs(x, residual, weight, eps):
+    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.shape[1] > 0,
+             "x must be a contiguous CUDA bf16 [M,C] tensor")
+    _require_vector(weight, x, x.shape[1], torch.bfloat16, "weight")
+    _require(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
+    if residual is None:
+        return x
+    _require(residual.is_cuda and residual.device == x.device and residual.dtype == torch.bfloat16
+             and residual.shape == x.shape and residual.is_contiguous(),
+             "residual must be a contiguous bf16 tensor of x's shape on the same device")
+    return torch.empty_like(x)
+
+
+def rmsnorm_residual_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6):
+    """sum = bf16(x + residual), y = sum / sqrt(mean(sum^2) + eps) * weight in fp32, quantised to
+    int8 rows in the same pass: [q int8 [M,C], scale fp32 [M,1], sum bf16 [M,C]] with
+    scale = max(max|y| / 127, 1e-30) and q = round half even(y / scale).  Without a residual, sum
+    is x itself."""
+    total = _rmsnorm_inputs(x, residual, weight, eps)
+    m, c = x.shape
+    q = torch.empty((m, c), dtype=torch.int8, device=x.device)
+    s = torch.empty((m, 1), dtype=torch.float32, device=x.device)
+    if m:
+        _call("b2_rmsnorm_residual_quant", x, x.data_ptr(), _ptr(residual), weight.data_ptr(),
+              None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+              work=("hbm", (3 if residual is None else 7) * m * c + 4 * m))
+    return [q, s, total]
+
+
+def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6):
+    """rmsnorm_residual_quant with an MXFP4 output: [q uint8 [M,C/2], scales uint8, sum bf16 [M,C]].
+    C must be a multiple of 32, at most 16384."""
+    total = _rmsnorm_inputs(x, residual, weight, eps)
+    m, c = x.shape
+    _require(c % MX_BLOCK == 0 and c <= 16384, f"the width must be a multiple of {MX_BLOCK}, at most 16384")
+    q, s = _mx_empty(m, c, x.device)
+    if m:
+        _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), _ptr(residual), weight.data_ptr(),
+              None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+              work=("hbm", (2 if residual is None else 6) * m * c + m * c // 2 + m * c // MX_BLOCK))
+    return [q, s, total]
+
+
 def check_device_status(device=None) -> None:
     """Synchronise and raise if a bounded device-side wait gave up (on `device`, default:
     the current device; the status word lives in each device's copy of the library image)."""

@@ -263,6 +263,52 @@ int b2_images_to_u8(const void* images, int32_t dtype, uint8_t* out, int64_t n, 
 int b2_gate_residual(void* x_bf16, const void* y_bf16, const void* gate_bf16, int64_t M, int64_t C,
                      void* stream);
 
+/* ---- Microscaled 4-bit floating point (MXFP4): quantiser, product and their values --------
+ * No counterpart in the reference; the next format below its rowwise INT8 linears.
+ *
+ * 32 consecutive columns of a row share a power-of-two scale 2^e, e = floor(log2(max|x|)) - 2
+ * within [-127, 127] (-127 for a block of zeros), stored as the byte e + 127; the elements are
+ * x / 2^e rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, ties to the even code,
+ * saturating at 6, two per byte with the even column in the low half.  A block with a NaN or an
+ * infinity has the scale byte 255 (NaN) and zero elements.
+ *   q       uint8 [M, K/2]
+ *   scales  uint8 [ceil(M/128)][ceil(K/128)][512]: the byte of row r and block b of a tile is
+ *           (r % 32) * 16 + (r / 32) * 4 + b.  The quantisers write every byte, those outside the
+ *           matrix as 0; bytes of blocks at or beyond K must not be 255 when scales come from
+ *           elsewhere.
+ * K must be a multiple of 32.  Pointers are 16-byte aligned. */
+
+/* x bf16 [M,K] contiguous. */
+int b2_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, void* stream);
+/* x bf16 [M,2K], gate columns then up columns: quantises silu(gate) * up, computed in fp32. */
+int b2_swiglu_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, void* stream);
+/* out bf16 [M,K]: the values (exact, except where 6 * 2^e leaves bf16's range). */
+int b2_dequantize_mxfp4(const uint8_t* q, const uint8_t* scales, void* out, int64_t M, int64_t K, void* stream);
+/* out bf16 [M,K] = bf16(q * scale[row]): the values of rowwise int8. */
+int b2_dequantize_int8_rowwise(const int8_t* q, const float* scale, void* out, int64_t M, int64_t K, void* stream);
+
+/* out bf16 [M,N] = bf16(a [M,K] . w [N,K]^T + bias), products and sums in fp32 on the tensor
+ * core, one rounding.  N must be a multiple of 8. */
+int b2_mxfp4_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* w, const uint8_t* w_scales,
+                  const void* bias, int bias_kind, void* out, int64_t M, int64_t N, int64_t K, void* stream);
+/* (activation) -> quantise -> product in one call; q_scratch and s_scratch are sized as q and
+ * scales of an [M,K] matrix above. */
+int b2_mxfp4_linear(const void* x, int input_act, const uint8_t* w, const uint8_t* w_scales, const void* bias,
+                    int bias_kind, void* out, uint8_t* q_scratch, uint8_t* s_scratch, int64_t M, int64_t N,
+                    int64_t K, void* stream);
+
+/* RMSNorm with the residual's addition and a quantised output (no counterpart in the reference):
+ *   sum = bf16(x + residual);  y = sum / sqrt(mean(sum^2) + eps) * weight in fp32
+ * x, residual, sum bf16 [M,C], weight bf16 [C].  residual and sum may both be null: the norm of x.
+ * sum must not alias an input.
+ * _quant: q int8 [M,C], scale fp32 [M] = max(max|y| / 127, 1e-30), q = round half even(y / scale);
+ *   a row with a NaN or an infinity keeps it in its scale and has zero elements.  Any C.
+ * _mxfp4: q and scales as above, C a multiple of 32, at most 16384. */
+int b2_rmsnorm_residual_quant(const void* x, const void* residual, const void* weight, void* sum, int8_t* q,
+                              float* scale, int64_t M, int64_t C, float eps, void* stream);
+int b2_rmsnorm_residual_mxfp4(const void* x, const void* residual, const void* weight, void* sum, uint8_t* q,
+                              uint8_t* scales, int64_t M, int64_t C, float eps, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
