@@ -58,6 +58,8 @@ SYMBOLS = {
     "b2_dequantize_int8_rowwise": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "b2_mxfp4_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp]),
     "b2_mxfp4_linear": (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "b2_window_fwd_workspace": (_int, [_i32] * 8 + [_vp]),
+    "b2_window_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp] + [_i32] * 5 + [_i64] * 9 + [_f32] + [_i32] * 3 + [_vp]),
     "b2_rmsnorm_residual_quant": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
     "b2_rmsnorm_residual_mxfp4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
 }

@@ -67,7 +67,7 @@ int b2_check_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "stream synchronize: %s", cudaGetErrorString(e));
   const unsigned int word = read_clear_status_gemm() | read_clear_status_gemm2() | read_clear_status_flash() |
-                            read_clear_status_flash2() | read_clear_status_mxfp4();
+                            read_clear_status_flash2() | read_clear_status_mxfp4() | read_clear_status_window();
   if (word == 0xffffffffu) return fail(B2_LAUNCH_FAILED, "status word could not be read");
   if (word != 0) return fail(B2_TIMEOUT, "device-side bounded wait gave up (code 0x%x)", word);
   return B2_OK;
@@ -458,6 +458,61 @@ int b2_mxfp4_linear(const void* x, int input_act, const uint8_t* w, const uint8_
   st = launch_quantize_mxfp4(x, q_scratch, s_scratch, M, K, input_act == B2_ACT_SWIGLU, (cudaStream_t)stream);
   if (st != B2_OK) return st;
   return launch_mxfp4_gemm(q_scratch, s_scratch, w, w_scales, bias, bias_kind, out, M, N, K, (cudaStream_t)stream);
+}
+
+static int check_window_sizes(int32_t B, int32_t H, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t left, int32_t right,
+                              int32_t sinks) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Sk <= 0)
+    return fail(B2_BAD_SHAPE, "window_fwd: batch, heads, and sequence lengths must be positive");
+  if (H % Hkv != 0) return fail(B2_BAD_SHAPE, "window_fwd: %d query heads are no multiple of %d key heads", H, Hkv);
+  if (left < -1 || right < -1 || sinks < 0)
+    return fail(B2_BAD_SHAPE, "window_fwd: left and right must be at least -1 (no limit), sinks at least 0");
+  if (Hkv > 65535 || B > 65535) return fail(B2_TOO_LARGE, "window_fwd: heads/batch exceed the launch grid");
+  if ((int64_t)Sq * H > 0x3fffffffLL || Sk > 0x3fffffff) return fail(B2_TOO_LARGE, "window_fwd: sequence too long");
+  return B2_OK;
+}
+
+int b2_window_fwd_workspace(int32_t B, int32_t H, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t left, int32_t right,
+                            int32_t sinks, int64_t* bytes) {
+  B2_REQUIRE_PTR(bytes);
+  const int st = check_window_sizes(B, H, Hkv, Sq, Sk, left, right, sinks);
+  if (st != B2_OK) return st;
+  *bytes = window_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, left, right, sinks);
+  return B2_OK;
+}
+
+int b2_window_fwd(const void* q, const void* k, const void* v, void* out, void* workspace, int64_t workspace_bytes,
+                  const int32_t* kv_lengths, int32_t B, int32_t H, int32_t Hkv, int32_t Sq, int32_t Sk, int64_t qsb,
+                  int64_t qsh, int64_t qss, int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
+                  int64_t vss, float scale, int32_t left, int32_t right, int32_t sinks, void* stream) {
+  const int st = check_window_sizes(B, H, Hkv, Sq, Sk, left, right, sinks);
+  if (st != B2_OK) return st;
+  if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(B2_BAD_SHAPE, "window_fwd: softmax_scale must be finite and positive");
+  if (!q || !k || !v || !out) return fail(B2_NULL_POINTER, "window_fwd: null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(kv_lengths) & 3u))
+    return fail(B2_BAD_STRIDE, "window_fwd: pointers must be 16-byte aligned");
+  int64_t qs[3] = {qsb, qsh, qss}, ks[3] = {ksb, ksh, kss}, vs[3] = {vsb, vsh, vss};
+  const int64_t kv_extent[3] = {B, Hkv, Sk}, q_extent[3] = {B, H, Sq};
+  for (int t = 0; t < 3; ++t) {
+    int64_t* s = t == 0 ? qs : t == 1 ? ks : vs;
+    const int64_t* extent = t == 0 ? q_extent : kv_extent;
+    for (int d = 2; d >= 0; --d) {
+      if (extent[d] == 1) {   // the stride of a single entry has no meaning: the next one's extent
+        s[d] = d == 2 ? 128 : s[d + 1] * extent[d + 1];
+        continue;
+      }
+      if (s[d] <= 0) return fail(B2_BAD_STRIDE, "window_fwd: strides must be positive");
+      if (s[d] % 8 != 0) return fail(B2_BAD_STRIDE, "window_fwd: strides must be multiples of 8 elements (16 bytes)");
+      if (s[d] < 128) return fail(B2_BAD_STRIDE, "window_fwd: stride below the head dimension");
+      if (s[d] >= (1LL << 38)) return fail(B2_TOO_LARGE, "window_fwd: stride too large");
+    }
+  }
+  const int64_t need = window_fwd_workspace_bytes(B, H, Hkv, Sq, Sk, left, right, sinks);
+  if (need > workspace_bytes || (need > 0 && workspace == nullptr))
+    return fail(B2_BAD_SHAPE, "window_fwd: the workspace has %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+  return launch_window_fwd(q, k, v, out, workspace, kv_lengths, B, H, Hkv, Sq, Sk, qs, ks, vs, scale, left, right, sinks,
+                           (cudaStream_t)stream);
 }
 
 }  // extern "C"

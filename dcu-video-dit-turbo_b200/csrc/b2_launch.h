@@ -73,6 +73,12 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* sum, void* q, void* scale,
                             int64_t M, int64_t C, float eps, bool mx, cudaStream_t stream);
 
+// Attention with a sliding window and first keys that stay visible (strides in elements, [b, h, s]).
+int64_t window_fwd_workspace_bytes(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks);
+int launch_window_fwd(const void* q, const void* k, const void* v, void* out, void* workspace, const int* lengths,
+                      int B, int H, int Hkv, int Sq, int Sk, const int64_t* qs, const int64_t* ks, const int64_t* vs,
+                      float scale, int left, int right, int sinks, cudaStream_t stream);
+
 int launch_bounded_wait_selftest(cudaStream_t stream);
 // Read and clear the device-side status word of a tensor-core translation unit.
 unsigned int read_clear_status_gemm();
@@ -80,5 +86,6 @@ unsigned int read_clear_status_gemm2();
 unsigned int read_clear_status_flash();
 unsigned int read_clear_status_flash2();
 unsigned int read_clear_status_mxfp4();
+unsigned int read_clear_status_window();
 
 }  // namespace b2

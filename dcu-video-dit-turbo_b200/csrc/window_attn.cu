@@ -1,0 +1,716 @@
+// bf16 attention with a sliding window and a few first keys that stay visible, for sm_100a: shared
+// key heads, queries that sit at the end of a longer key sequence (a cache), per-sequence lengths.
+//
+// Query i of a sequence with n keys sits at p = i + n - Sq and sees the keys j < n with
+//   j <= p + right   and   (j >= p - left  or  j < sinks)
+// (left, right < 0: no limit on that side).  A query that sees nothing gives zeros.
+//
+// The mathematics is flash_fwd.cu's (exp2-domain running softmax in fp32, a fixed share of the
+// exponentials on the FMA pipe, rescaling only when the running maximum grows by more than 2^8);
+// flash_common.cuh holds the shared pieces.  What differs:
+//
+//   rows      The H / Hkv query heads that share a key head are packed with the positions, row
+//             r = i * (H / Hkv) + head, so a CTA's rows read one set of keys and span few positions.
+//             Rows are fetched with plain 16-byte loads into the swizzled tile (any strides, any
+//             packing).
+//   keys      A CTA walks only the 128-key tiles that some row of it sees: the tiles of the first
+//             keys, then those of its window.  Scores are masked in the tiles that some row does
+//             not see whole ("mixed"); the others take flash_fwd.cu's path.
+//   values    0 * NaN is NaN, so a value that a row must not see may not meet its zero weight in a
+//             product: the two otherwise idle warps look through every mixed tile, clear the rows
+//             at or past n (a cache's unwritten part) and set non-finite values to zero.  Those of
+//             visible keys are added back to the rows that see them at the end (a path that only
+//             runs if there were any).
+//   few rows  With at most 128 rows per key head (single tokens) the two query tiles become two
+//             streams over the same rows: stream 0 takes the even tiles, stream 1 the odd ones, and
+//             the key sequence is split over CTAs as well.  Each stream leaves its maximum, sum and
+//             unnormalised output; a second kernel joins them.  Larger calls whose grid would leave
+//             SMs empty are split the same way.
+//
+// Bound by the tensor cores (4 * 128 FLOP per visible pair and head) when many rows share the keys,
+// by reading K and V once for single tokens.
+#include "flash_common.cuh"
+
+namespace b2 {
+
+unsigned int read_clear_status_window() { return read_and_clear_device_status(); }
+
+namespace {
+
+using namespace flash;
+
+constexpr int WIN_REGS_SERVICE = 40;
+static_assert(2 * B2_FLASH_REGS_SOFTMAX + WIN_REGS_SERVICE <= 3 * kLaunchRegs,
+              "register split exceeds the CTA's launch allocation");
+constexpr int KV_STAGES = 2;
+constexpr int SMEM_Q = 0;
+constexpr int SMEM_K = SMEM_Q + 2 * TILE_BYTES;
+constexpr int SMEM_V = SMEM_K + KV_STAGES * TILE_BYTES;
+constexpr int SMEM_BARS = SMEM_V + KV_STAGES * TILE_BYTES;
+constexpr int WV_CLEAN = NUM_BARS;                    // [stage]: a mixed tile's values are cleared
+constexpr int WIN_BARS = NUM_BARS + KV_STAGES;
+constexpr int SMEM_TOTAL = 1024 + SMEM_BARS + WIN_BARS * 8 + 16;
+constexpr int kFixWarp = 10, kFixThreads = 64;
+
+struct WinArgs {
+  __nv_bfloat16* out;           // [B, Sq, H, 128]
+  float* part_o;                // [parts][B * Sq * H][128], null: no parts
+  float2* part_ml;              // [parts][B * Sq * H]: (maximum in the exp2 domain, sum)
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* v;       // for the non-finite path
+  const int* lengths;           // keys per sequence, null: Sk
+  int64_t q_b, q_h, q_s, v_b, v_h, v_s;   // strides in elements
+  int H, Hkv, share, Sq, Sk, rows;        // share = H / Hkv, rows = Sq * share
+  int left, right, sinks, splits;
+  int64_t total_rows;                     // B * Sq * H
+  int k_swap, v_swap;
+  float scale_log2;
+};
+
+// What a CTA reads: the same numbers in every role.
+struct Span {
+  int n;                 // keys of this sequence
+  int p_min, p_max;      // positions of its rows
+  int sink_tiles, win0;  // steps 0..sink_tiles-1 are tiles 0.., the others win0..
+  int step0, steps;      // this CTA's share of the steps
+};
+
+__device__ __forceinline__ int sequence_keys(const int* lengths, int b, int Sk) {
+  return lengths == nullptr ? Sk : min(max(lengths[b], 0), Sk);
+}
+// j <= p + right with no limit for right < 0; positions and limits stay below 2^31 (checked by the
+// entry point), the sum may not
+__device__ __forceinline__ int last_key(int p, int right, int n) {
+  return right < 0 ? n - 1 : (int)min((int64_t)p + right, (int64_t)n - 1);
+}
+__device__ __forceinline__ int first_key(int p, int left) {
+  return left < 0 ? 0 : max((int)max((int64_t)p - left, (int64_t)-1), 0);
+}
+
+template <int ROWS>
+__device__ __forceinline__ Span make_span(const WinArgs& a, int row0, int b, int split) {
+  Span s;
+  s.n = sequence_keys(a.lengths, b, a.Sk);
+  const int last_row = min(row0 + ROWS, a.rows) - 1;
+  s.p_min = row0 / a.share + s.n - a.Sq;
+  s.p_max = last_row / a.share + s.n - a.Sq;
+  const int end = last_key(s.p_max, a.right, s.n) + 1;           // <= 0: nothing is visible
+  const int begin = first_key(s.p_min, a.left);
+  int total = 0;
+  s.sink_tiles = s.win0 = 0;
+  if (end > 0) {
+    s.win0 = begin / BLOCK_N;
+    s.sink_tiles = min((min(a.sinks, end) + BLOCK_N - 1) / BLOCK_N, s.win0);
+    total = s.sink_tiles + max((end + BLOCK_N - 1) / BLOCK_N - s.win0, 0);
+  }
+  s.step0 = (int)((int64_t)total * split / a.splits);
+  s.steps = (int)((int64_t)total * (split + 1) / a.splits) - s.step0;
+  return s;
+}
+// first key of the CTA's step j
+__device__ __forceinline__ int step_key(const Span& s, int j) {
+  const int g = s.step0 + j;
+  return (g < s.sink_tiles ? g : s.win0 + g - s.sink_tiles) * BLOCK_N;
+}
+// some row of the CTA does not see the whole tile
+__device__ __forceinline__ bool is_mixed(const WinArgs& a, const Span& s, int key0) {
+  return key0 + BLOCK_N - 1 > last_key(s.p_min, a.right, s.n) ||
+         (key0 < first_key(s.p_max, a.left) && key0 + BLOCK_N > a.sinks);
+}
+__device__ __forceinline__ bool sees_any(const WinArgs& a, int p, int n) {
+  const int last = last_key(p, a.right, n);
+  return last >= 0 && (last >= first_key(p, a.left) || a.sinks > 0);
+}
+
+constexpr uint32_t kIdescQK = make_idesc(/*f32*/ 1, /*bf16*/ 1, /*bf16*/ 1, 0, 0, BLOCK_M, BLOCK_N);
+constexpr uint32_t kIdescPV = make_idesc(1, 1, 1, 0, /*B MN-major*/ 1, BLOCK_M, HEAD_DIM);
+
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row0, int h,
+                                          int b, int swap) {
+  mbar_expect_tx(bar, TILE_BYTES);
+  if (swap) {
+    tma_load_4d(dst, map, bar, 0, h, row0, b);
+    tma_load_4d(dst + HALF_BYTES, map, bar, 64, h, row0, b);
+  } else {
+    tma_load_4d(dst, map, bar, 0, row0, h, b);
+    tma_load_4d(dst + HALF_BYTES, map, bar, 64, row0, h, b);
+  }
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t max_bits4(uint32_t m, const uint4& v) {
+  m = __vmaxu2(m, v.x & 0x7fff7fffu);
+  m = __vmaxu2(m, v.y & 0x7fff7fffu);
+  m = __vmaxu2(m, v.z & 0x7fff7fffu);
+  return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0u : 0xffffu, hi = (w & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
+  return w & (lo | hi);
+}
+
+// A mixed tile of values: rows at or past `valid` become zeros, non-finite values become zeros;
+// returns whether a row before `valid` held one.  64 threads, one 128-byte line half at a time.
+__device__ __forceinline__ bool clean_values(uint32_t tile, int valid, int ft) {
+  bool found = false;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    // thread ft owns lines ft and ft + 64 of the half tile; the order of the 16-byte chunks differs
+    // from thread to thread so that the eight lanes of a phase touch different banks
+#pragma unroll 1
+    for (int l = 0; l < 2; ++l) {
+      const int row = ft + 64 * l;
+      const uint32_t line = tile + half * HALF_BYTES + row * 128;
+      if (row >= valid) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sts128(line + ((c ^ (row & 7)) << 4), make_uint4(0, 0, 0, 0));
+        continue;
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) m = max_bits4(m, lds128(line + ((c ^ (row & 7)) << 4)));
+      if ((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) {
+        found = true;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint4 v = lds128(line + (c << 4));
+          v.x = finite_or_zero(v.x);
+          v.y = finite_or_zero(v.y);
+          v.z = finite_or_zero(v.z);
+          v.w = finite_or_zero(v.w);
+          sts128(line + (c << 4), v);
+        }
+      }
+    }
+  }
+  return found;
+}
+
+// FEW: at most 128 rows per key head; the two tiles are two streams over the same rows.
+template <bool FEW>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                  const __grid_constant__ WinArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WIN_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* nonfinite = abort_flag + 1;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int idx) -> uint32_t { return bar0 + idx * 8; };
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  constexpr int CTA_ROWS = FEW ? BLOCK_M : 2 * BLOCK_M;
+  // the last rows of a causal call see the most keys: they start first
+  const int block = gridDim.x / args.splits - 1 - blockIdx.x / args.splits;
+  const int split = blockIdx.x % args.splits;
+  const int hkv = blockIdx.y, b = blockIdx.z;
+  const int row0 = block * CTA_ROWS;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < WIN_BARS; ++i) {
+      int count = 1;
+      if (i == Q_FULL || i == Q_FULL + 1) count = 4;                     // the tile's four warps
+      if (i >= P_PART && i < P_PART + 2 * P_PARTS) count = 4;
+      if (i == V_EMPTY || i == V_EMPTY + 1) count = 1 + kFixThreads / 32;   // MMAs done, looked through
+      if (i >= WV_CLEAN) count = kFixThreads;
+      mbar_init(bar(i), count);
+    }
+    *abort_flag = 0;
+    *nonfinite = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const Span span = make_span<CTA_ROWS>(args, row0, b, split);
+  const int steps = span.steps;
+
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WIN_REGS_SERVICE));
+    if (warp == kLoadWarp) {
+      if (lane == 0) {
+        for (int j = 0; j < steps; ++j) {
+          const int st = j & 1;
+          const uint32_t par = ((j >> 1) & 1) ^ 1;
+          const int key0 = step_key(span, j);
+          if (!mbar_wait(bar(K_EMPTY + st), par, abort_flag, kStatusFlashTimeout)) break;
+          load_tile(sbase + SMEM_K + st * TILE_BYTES, &tmap_k, bar(K_FULL + st), key0, hkv, b, args.k_swap);
+          if (!mbar_wait(bar(V_EMPTY + st), par, abort_flag, kStatusFlashTimeout)) break;
+          load_tile(sbase + SMEM_V + st * TILE_BYTES, &tmap_v, bar(V_FULL + st), key0, hkv, b, args.v_swap);
+        }
+      }
+    } else if (warp >= kFixWarp) {
+      const int ft = threadIdx.x - kFixWarp * 32;
+      // every step is waited for and released, mixed or not: these warps can neither run ahead of
+      // the ring by a whole phase nor fall behind it by one
+      for (int j = 0; j < steps; ++j) {
+        const int key0 = step_key(span, j);
+        const int st = j & 1;
+        if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1, abort_flag, kStatusFlashTimeout)) break;
+        if (is_mixed(args, span, key0)) {
+          if (clean_values(sbase + SMEM_V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
+          fence_proxy_async_smem();
+          mbar_arrive(bar(WV_CLEAN + st));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(V_EMPTY + st));
+      }
+    } else if (warp == kMmaWarp && steps > 0) {
+      const bool leader = elect_one() != 0;
+      const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // tile 1: 128 columns on
+      const uint32_t q0 = desc_lo(sbase + SMEM_Q, 16);
+      const uint32_t k0 = desc_lo(sbase + SMEM_K, 16);
+      const uint32_t v0 = desc_lo(sbase + SMEM_V, HALF_BYTES);
+      constexpr uint32_t TILE_UNITS = TILE_BYTES >> 4;
+      uint32_t clean_phase = 0;   // bit per stage
+      // S of tile t = Q . K^T of the stage's keys
+      auto issue_qk = [&](int t, int st) {
+        if (leader) mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + (FEW ? 0 : t) * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
+        if (leader) tc_commit(bar(S_FULL + t));
+      };
+      // the stage's values are there, and cleared if the tile is mixed
+      auto wait_v = [&](int j) -> bool {
+        const int st = j & 1;
+        if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1, abort_flag, kStatusFlashTimeout)) return false;
+        if (is_mixed(args, span, step_key(span, j))) {
+          if (!mbar_wait(bar(WV_CLEAN + st), (clean_phase >> st) & 1, abort_flag, kStatusFlashTimeout)) return false;
+          clean_phase ^= 1u << st;
+        }
+        return true;
+      };
+      // O of tile t += P . V, each half of P as soon as it is published; `use` counts the tile's steps
+      auto issue_pv = [&](int t, int st, int use) -> bool {
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!mbar_wait(bar(P_PART + 2 * part + t), use & 1, abort_flag, kStatusFlashTimeout)) return false;
+          tc_fence_after();
+          if (leader) {
+            if (part == 0)
+              mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, use != 0 ? 1u : 0u);
+            else
+              mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
+          }
+        }
+        return true;
+      };
+      static_assert(P_PARTS == 2, "P is published in halves");
+      bool ok = mbar_wait(bar(Q_FULL), 0, abort_flag, kStatusFlashTimeout) &&
+                mbar_wait(bar(K_FULL), 0, abort_flag, kStatusFlashTimeout);
+      if constexpr (FEW) {
+        // step j belongs to stream j & 1, which is also its ring stage
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, 0);
+          if (leader) tc_commit(bar(K_EMPTY));
+        }
+        if (ok && steps > 1) {
+          ok = mbar_wait(bar(K_FULL + 1), 0, abort_flag, kStatusFlashTimeout);
+          if (ok) {
+            issue_qk(1, 1);
+            if (leader) tc_commit(bar(K_EMPTY + 1));
+          }
+        }
+        for (int j = 0; ok && j < steps; ++j) {
+          const int t = j & 1;
+          if (!(ok = wait_v(j) && issue_pv(t, t, j >> 1))) break;
+          if (leader) tc_commit(bar(V_EMPTY + t));
+          if (j + 2 < steps) {
+            if (!(ok = mbar_wait(bar(K_FULL + t), ((j + 2) >> 1) & 1, abort_flag, kStatusFlashTimeout))) break;
+            tc_fence_after();
+            issue_qk(t, t);
+            if (leader) tc_commit(bar(K_EMPTY + t));
+          } else {
+            if (leader) tc_commit(bar(O_FULL + t));
+          }
+        }
+      } else {
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, 0);
+          ok = mbar_wait(bar(Q_FULL + 1), 0, abort_flag, kStatusFlashTimeout);
+        }
+        if (ok) {
+          tc_fence_after();
+          issue_qk(1, 0);
+          if (leader) tc_commit(bar(K_EMPTY));
+          ok = wait_v(0);
+        }
+        for (int j = 0; ok && j < steps; ++j) {
+          const int st = j & 1;
+          const bool last = j + 1 == steps;
+          if (!(ok = issue_pv(0, st, j))) break;
+          if (last) {
+            if (leader) tc_commit(bar(O_FULL));
+          } else {
+            if (!(ok = mbar_wait(bar(K_FULL + (st ^ 1)), ((j + 1) >> 1) & 1, abort_flag, kStatusFlashTimeout))) break;
+            tc_fence_after();
+            issue_qk(0, st ^ 1);
+          }
+          if (!(ok = issue_pv(1, st, j))) break;
+          if (leader) tc_commit(bar(V_EMPTY + st));
+          if (last) {
+            if (leader) tc_commit(bar(O_FULL + 1));
+          } else {
+            // the next step's values, waited for while this step's MMAs are still queued
+            if (!(ok = wait_v(j + 1))) break;
+            issue_qk(1, st ^ 1);
+            if (leader) tc_commit(bar(K_EMPTY + (st ^ 1)));
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(B2_FLASH_REGS_SOFTMAX));
+    const int t = warp >> 2;
+    const int quarter = warp & 3;
+    const int tile_row0 = row0 + (FEW ? 0 : t * BLOCK_M);
+    if (steps > 0 && (!FEW || t == 0)) {
+      // this tile's rows of Q: 16 lanes per row, all loads in flight before the first store
+      const int tid = threadIdx.x & 127, c16 = tid & 15;
+      uint4 v[16];
+#pragma unroll
+      for (int p = 0; p < 16; ++p) {
+        const int r = tile_row0 + p * 8 + (tid >> 4);
+        v[p] = make_uint4(0, 0, 0, 0);
+        if (r < args.rows) {
+          const int i = r / args.share, h = hkv * args.share + (r - i * args.share);
+          v[p] = ldg_stream(reinterpret_cast<const uint4*>(args.q + b * args.q_b + h * args.q_h + i * args.q_s) + c16);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 16; ++p) {
+        const int r = p * 8 + (tid >> 4);
+        sts128(sbase + SMEM_Q + t * TILE_BYTES + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Q_FULL + t));
+    }
+    const int uses = FEW ? (steps + 1 - t) >> 1 : steps;   // steps of this tile (stream)
+    const int row = tile_row0 + quarter * 32 + lane;
+    const bool row_ok = row < args.rows;
+    const bool warp_ok = tile_row0 + quarter * 32 < args.rows;
+    const int my_row = min(row, args.rows - 1);
+    const int my_i = my_row / args.share;
+    const int p_row = my_i + span.n - args.Sq;
+    const int key_last = last_key(p_row, args.right, span.n);
+    const int key_first = first_key(p_row, args.left);
+    const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem_base + COL_S0 + t * 128 + lane_sel;
+    const uint32_t p_tmem = s_tmem;
+    const uint32_t o_tmem = tmem_base + COL_O0 + t * 128 + lane_sel;
+    const float sl2 = args.scale_log2;
+    bool ok = true;
+    float row_max = -INFINITY, row_sum = 0.f;
+    for (int u = 0; u < uses; ++u) {
+      if (ok) ok = mbar_wait(bar(S_FULL + t), u & 1, abort_flag, kStatusFlashTimeout);
+      tc_fence_after();
+      if (!warp_ok) {   // none of the warp's rows exist: whatever P holds there goes nowhere
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(P_PART + t));
+          mbar_arrive(bar(P_PART + 2 + t));
+        }
+        continue;
+      }
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld_32x32b_x32(s_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+      tmem_wait_ld();
+      {
+        // visible columns: [first, last] and those before `sink`
+        const int key0 = step_key(span, FEW ? 2 * u + t : u);
+        const int last = key_last - key0, first = key_first - key0, sink = args.sinks - key0;
+        if (__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N))) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c > last || (c < first && c >= sink)) s[c] = 0xff800000u;   // -inf
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; c += 2)
+        mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+      const float m_row = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool raise = (m_row - row_max) * sl2 > 8.0f;   // false while both are -inf (NaN)
+      float alpha = 1.0f;
+      if (raise) {
+        alpha = ex2_approx((row_max - m_row) * sl2);
+        row_max = m_row;
+        row_sum *= alpha;
+      }
+      if (u != 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(o_tmem + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st_32x32b_x16(o_tmem + c, o);
+        }
+      }
+      // a row that has seen nothing yet has only -inf scores: exp2(-inf - 0) = 0
+      const float neg_ms = row_max == -INFINITY ? 0.0f : -row_max * sl2;
+      const uint64_t sl2x2 = pack2(sl2, sl2), nmsx2 = pack2(neg_ms, neg_ms);
+      uint64_t sm2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        uint32_t p[8];
+        exp_chunk(&s[16 * q], p, sl2x2, nmsx2, sm2);
+        tmem_st_32x32b_x8(p_tmem + 8 * q, p);
+        if ((q + 1) % 4 == 0) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(P_PART + 2 * (q / 4) + t));
+        }
+      }
+      float a0, a1, b0, b1, c0, c1, d0, d1;
+      unpack2(sm2[0], a0, a1);
+      unpack2(sm2[1], b0, b1);
+      unpack2(sm2[2], c0, c1);
+      unpack2(sm2[3], d0, d1);
+      row_sum += ((a0 + a1) + (b0 + b1)) + ((c0 + c1) + (d0 + d1));
+    }
+    if (ok && uses > 0) ok = mbar_wait(bar(O_FULL + t), 0, abort_flag, kStatusFlashTimeout);
+    // without parts the few-row form has a single step, which is stream 0's
+    if (ok && warp_ok && !(FEW && t == 1 && args.part_o == nullptr)) {
+      tc_fence_after();
+      const int h = hkv * args.share + (my_row - my_i * args.share);
+      const int64_t out_row = ((int64_t)b * args.Sq + my_i) * args.H + h;
+      const bool parts = args.part_o != nullptr;
+      const int part = FEW ? 2 * split + t : split;
+      // keys in sight whose scores are all -inf leave 0 / 0, as the formula does
+      const float inv = parts ? 1.0f
+                        : row_sum == 0.f ? (sees_any(args, p_row, span.n) ? __uint_as_float(0x7fc00000u) : 0.0f)
+                        : row_sum != row_sum ? 1.0f : 1.0f / row_sum;
+      if (parts && row_ok)
+        args.part_ml[part * args.total_rows + out_row] = make_float2(row_max * sl2, row_sum);
+      const bool fix = *nonfinite != 0;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t o[32];
+        if (uses > 0) {
+          tmem_ld_32x32b_x32(o_tmem + c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (fix && row_ok) {
+          for (int u = 0; u < uses; ++u) {
+            const int key0 = step_key(span, FEW ? 2 * u + t : u);
+            if (!is_mixed(args, span, key0)) continue;
+            for (int j = key0; j < key0 + BLOCK_N && j <= key_last; ++j) {
+              if (j < key_first && j >= args.sinks) continue;
+              const __nv_bfloat16* src = args.v + b * args.v_b + hkv * args.v_h + (int64_t)j * args.v_s + c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float x = __bfloat162float(src[i]);
+                if (!(fabsf(x) <= 3.4e38f)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+              }
+            }
+          }
+        }
+        if (!row_ok) continue;
+        if (parts) {
+          uint4* dst = reinterpret_cast<uint4*>(args.part_o + (part * args.total_rows + out_row) * HEAD_DIM + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(args.out + out_row * HEAD_DIM + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 w;
+            w.x = pack_bf16x2_rn(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+            w.y = pack_bf16x2_rn(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+            w.z = pack_bf16x2_rn(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+            w.w = pack_bf16x2_rn(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+            dst[i] = w;
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag != 0) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 200000) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// Joins the parts of each row: weights 2^(m - max m), one warp per row, four columns per lane.
+__global__ void __launch_bounds__(256)
+window_join_kernel(const WinArgs args, int parts) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= args.total_rows) return;
+  float top = -INFINITY;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, args.part_ml[p * args.total_rows + row].x);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool any_nan = false;
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = args.part_ml[p * args.total_rows + row];
+    any_nan |= ml.y != ml.y;
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;   // this part saw nothing
+    const float w = exp2f(ml.x - top);
+    const float4 x = reinterpret_cast<const float4*>(args.part_o + (p * args.total_rows + row) * HEAD_DIM)[lane];
+    l = fmaf(w, ml.y, l);
+    o.x = fmaf(w, x.x, o.x);
+    o.y = fmaf(w, x.y, o.y);
+    o.z = fmaf(w, x.z, o.z);
+    o.w = fmaf(w, x.w, o.w);
+  }
+  float inv = 1.0f / l;
+  if (any_nan) {
+    inv = __uint_as_float(0x7fc00000u);
+  } else if (l == 0.f) {
+    const int64_t bi = row / args.H;
+    const int b = (int)(bi / args.Sq), i = (int)(bi - (int64_t)b * args.Sq);
+    const int n = sequence_keys(args.lengths, b, args.Sk);
+    inv = sees_any(args, i + n - args.Sq, n) ? __uint_as_float(0x7fc00000u) : 0.f;
+  }
+  uint2 w;
+  w.x = pack_bf16x2_rn(o.x * inv, o.y * inv);
+  w.y = pack_bf16x2_rn(o.z * inv, o.w * inv);
+  reinterpret_cast<uint2*>(args.out + row * HEAD_DIM)[lane] = w;
+}
+
+// How a call is laid over the GPU: few-row form or not, splits of the key sequence, parts to join.
+struct WinPlan {
+  bool few;
+  int blocks, splits, parts;
+};
+WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks) {
+  WinPlan p;
+  const int share = H / Hkv;
+  const int64_t rows = (int64_t)Sq * share;
+  p.few = rows <= BLOCK_M;
+  const int cta_rows = p.few ? BLOCK_M : 2 * BLOCK_M;
+  p.blocks = (int)((rows + cta_rows - 1) / cta_rows);
+  // the most 128-key steps that a CTA can have: its rows' positions, the window around them, the
+  // first keys; one more for a window that starts inside a tile
+  const int64_t positions = min((int64_t)Sq, (int64_t)cta_rows / share + 2);
+  int64_t keys = Sk;
+  if (left >= 0 && right >= 0) keys = min(keys, (int64_t)left + right + positions);
+  int64_t steps = (keys + BLOCK_N - 1) / BLOCK_N + (keys < Sk ? 1 : 0);
+  if (left >= 0) steps += (min(sinks, Sk) + BLOCK_N - 1) / BLOCK_N;
+  steps = max((int64_t)1, min(steps, ((int64_t)Sk + BLOCK_N - 1) / BLOCK_N));
+  // One CTA runs per SM, so a grid takes ceil(CTAs / SMs) rounds of (steps / splits + a fixed part
+  // worth about three steps: set-up, first loads, output).  Splitting pays while it fills empty SMs.
+  const int64_t ctas = (int64_t)p.blocks * Hkv * B;
+  int64_t best = INT64_MAX;
+  p.splits = 1;
+  for (int s = 1; s <= 64 && s <= steps; ++s) {
+    const int64_t rounds = (ctas * s + kNumSMsB200 - 1) / kNumSMsB200;
+    // parts cost: writing and joining them, about two steps' time per call
+    const int64_t cost = rounds * ((steps + s - 1) / s + 3) + (s > 1 ? 2 : 0);
+    if (cost < best) {
+      best = cost;
+      p.splits = s;
+    }
+  }
+  p.parts = p.splits * (p.few ? 2 : 1);
+  if (p.few && steps == 1) p.parts = 1;   // the second stream has nothing
+  return p;
+}
+
+}  // namespace
+
+int64_t window_fwd_workspace_bytes(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks) {
+  const WinPlan p = make_plan(B, H, Hkv, Sq, Sk, left, right, sinks);
+  return p.parts == 1 ? 0 : (int64_t)p.parts * B * H * Sq * (HEAD_DIM * 4 + 8);
+}
+
+int launch_window_fwd(const void* q, const void* k, const void* v, void* out, void* workspace, const int* lengths,
+                      int B, int H, int Hkv, int Sq, int Sk, const int64_t* qs, const int64_t* ks, const int64_t* vs,
+                      float scale, int left, int right, int sinks, cudaStream_t stream) {
+  static PerDeviceSetup per_device;
+  const DeviceSlot* slot = nullptr;
+  const int setup_status = per_device.get("window_fwd", [](int, DeviceSlot&) -> int {
+    const void* kernels[2] = {(const void*)window_fwd_kernel<false>, (const void*)window_fwd_kernel<true>};
+    for (const void* f : kernels) {
+      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL);
+      if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "window_fwd: smem attribute: %s", cudaGetErrorString(e));
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, f);
+      if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "window_fwd: attributes: %s", cudaGetErrorString(e));
+      if (2 * B2_FLASH_REGS_SOFTMAX + WIN_REGS_SERVICE > 3 * ((fa.numRegs + 7) / 8 * 8))
+        return fail(B2_LAUNCH_FAILED, "window_fwd: register split %d/%d does not fit %d launch registers",
+                    B2_FLASH_REGS_SOFTMAX, WIN_REGS_SERVICE, fa.numRegs);
+    }
+    return B2_OK;
+  }, &slot);
+  if (setup_status != B2_OK) return setup_status;
+  const WinPlan plan = make_plan(B, H, Hkv, Sq, Sk, left, right, sinks);
+  CUtensorMap tk, tv;
+  WinArgs a;
+  int st = encode_qkv_map(&tk, k, B, Hkv, Sk, ks, &a.k_swap);
+  if (st != B2_OK) return st;
+  st = encode_qkv_map(&tv, v, B, Hkv, Sk, vs, &a.v_swap);
+  if (st != B2_OK) return st;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.total_rows = (int64_t)B * Sq * H;
+  a.part_o = plan.parts == 1 ? nullptr : reinterpret_cast<float*>(workspace);
+  a.part_ml = plan.parts == 1 ? nullptr : reinterpret_cast<float2*>(a.part_o + plan.parts * a.total_rows * HEAD_DIM);
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v);
+  a.lengths = lengths;
+  a.q_b = qs[0];
+  a.q_h = qs[1];
+  a.q_s = qs[2];
+  a.v_b = vs[0];
+  a.v_h = vs[1];
+  a.v_s = vs[2];
+  a.H = H;
+  a.Hkv = Hkv;
+  a.share = H / Hkv;
+  a.Sq = Sq;
+  a.Sk = Sk;
+  a.rows = Sq * a.share;
+  a.left = left;
+  a.right = right;
+  a.sinks = left < 0 ? 0 : sinks;
+  a.splits = plan.splits;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  const dim3 grid(plan.blocks * plan.splits, Hkv, B);
+  if (plan.few)
+    window_fwd_kernel<true><<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(tk, tv, a);
+  else
+    window_fwd_kernel<false><<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(tk, tv, a);
+  st = check_launch("window_fwd");
+  if (st != B2_OK || plan.parts == 1) return st;
+  window_join_kernel<<<(unsigned)((a.total_rows + 7) / 8), 256, 0, stream>>>(a, plan.parts);
+  return check_launch("window_fwd (join)");
+}
+
+}  // namespace b2

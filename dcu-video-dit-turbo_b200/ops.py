@@ -16,6 +16,7 @@ reference project:
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -750,6 +751,51 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
               None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
               work=("hbm", (2 if residual is None else 6) * m * c + m * c // 2 + m * c // MX_BLOCK))
     return [q, s, total]
+
+
+# ---- attention with a sliding window (no counterpart in the reference) --------------
+
+def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, left: int, right: int,
+                    sinks: int = 0, kv_lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 attention forward of q [B,H,Sq,128] over k, v [B,Hkv,Sk,128] (Hkv divides H; any
+    16-byte-aligned strides with a contiguous last dimension) with a window and first keys that stay
+    visible.  A sequence has n keys, `kv_lengths[b]` (int32 [B] on the same device, clamped to
+    [0, Sk]) or Sk; its query i sits at p = i + n - Sq and sees the keys j < n with j <= p + right
+    and (j >= p - left or j < sinks); -1 lifts the limit of a side (right=0: causal).  A query that
+    sees no key gives zeros, and what lies in keys or values that a query does not see has no effect
+    on it.  Returns the [B,H,Sq,128] transpose view of a fresh contiguous [B,Sq,H,128] tensor."""
+    _require(q.is_cuda and k.is_cuda and v.is_cuda, "q, k, and v must be on a CUDA device")
+    _require(q.dtype == torch.bfloat16, "kernel requires BF16 q")
+    _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, and v must have the same dtype")
+    _require(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, and v must use BHSD layout")
+    _require(q.device == k.device and q.device == v.device, "q, k, and v must be on the same CUDA device")
+    b, h, sq, d = q.shape
+    hkv, sk = k.shape[1], k.shape[2]
+    _require(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d,
+             "k and v must have the same shape and q's batch and head dimension")
+    _require(d == 128, "kernel requires head dimension 128")
+    _require(b > 0 and h > 0 and sq > 0 and hkv > 0 and sk > 0, "batch, heads, and sequence lengths must be positive")
+    _require(h % hkv == 0, "the query heads must be a multiple of the key heads")
+    _require(q.stride(3) == 1 and k.stride(3) == 1 and v.stride(3) == 1,
+             "q, k, and v must have contiguous last dimensions")
+    scale = float(softmax_scale)
+    _require(math.isfinite(scale) and scale > 0.0, "softmax_scale must be finite and positive")
+    left, right, sinks = int(left), int(right), int(sinks)
+    _require(left >= -1 and right >= -1 and sinks >= 0, "left and right must be at least -1, sinks at least 0")
+    # nothing lies further away than the sequences are long
+    left, right, sinks = min(left, sk + sq), min(right, sk + sq), min(sinks, sk)
+    if kv_lengths is not None:
+        _require_vector(kv_lengths, q, b, torch.int32, "kv_lengths")
+    storage = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+    need = ctypes.c_int64(0)
+    _lib.check(_lib.load().b2_window_fwd_workspace(b, h, hkv, sq, sk, left, right, sinks, ctypes.byref(need)),
+               "b2_window_fwd_workspace")
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    span = sk if left < 0 or right < 0 else min(sk, left + right + 1)
+    _call("b2_window_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), storage.data_ptr(), _ptr(workspace), need.value,
+          _ptr(kv_lengths), b, h, hkv, sq, sk, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], scale, left, right,
+          sinks, _stream(q), launches=2 if need.value else 1, work=("bf16", 4 * b * h * sq * span * d))
+    return storage.transpose(1, 2)
 
 
 def check_device_status(device=None) -> None:

@@ -309,6 +309,25 @@ int b2_rmsnorm_residual_quant(const void* x, const void* residual, const void* w
 int b2_rmsnorm_residual_mxfp4(const void* x, const void* residual, const void* weight, void* sum, uint8_t* q,
                               uint8_t* scales, int64_t M, int64_t C, float eps, void* stream);
 
+/* Attention with a sliding window and first keys that stay visible (no counterpart in the
+ * reference, whose attention is full).  q bf16 [B,H,Sq,128], k, v bf16 [B,Hkv,Sk,128], Hkv divides
+ * H (head h reads key head h / (H / Hkv)), each with its own [b, h, s] strides in elements
+ * (positive, multiples of 8, at least 128; ignored where the extent is 1); out bf16 [B,Sq,H,128]
+ * contiguous.
+ * A sequence has n keys: kv_lengths[b] (int32 on the device, clamped to [0, Sk]) or, with
+ * kv_lengths null, Sk.  Its query i sits at p = i + n - Sq and sees the keys j < n with
+ *   j <= p + right  and  (j >= p - left or j < sinks);
+ * left / right = -1: no limit on that side.  A query that sees no key gives zeros.  What lies in
+ * keys and values that a query does not see (NaN and infinities included) has no effect on it.
+ * workspace: b2_window_fwd_workspace's bytes, 16-byte aligned, in use until the call's kernels
+ * are done (0 bytes for many calls; null is then fine). */
+int b2_window_fwd_workspace(int32_t B, int32_t H, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t left, int32_t right,
+                            int32_t sinks, int64_t* bytes);
+int b2_window_fwd(const void* q, const void* k, const void* v, void* out, void* workspace, int64_t workspace_bytes,
+                  const int32_t* kv_lengths, int32_t B, int32_t H, int32_t Hkv, int32_t Sq, int32_t Sk, int64_t qsb,
+                  int64_t qsh, int64_t qss, int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
+                  int64_t vss, float scale, int32_t left, int32_t right, int32_t sinks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,3 +84,35 @@ def test_plain_mxfp4_follows_the_definition():
     assert torch.equal(R.mx_bytes(R.mx_tiles(byte), 300, 288), byte)
     codes = torch.randint(0, 16, (5, 64))
     assert torch.equal(R.mx_codes(R.mx_pack(codes)), codes)
+
+
+def test_window_arguments_are_checked_before_launch(pkg):
+    lib = pkg._lib.load()
+    s = [1 << 20, 128, 128 * 4]
+    good = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, ws=None, ws_bytes=0, lengths=None, B=1, H=4, Hkv=4, Sq=512, Sk=512, qs=s, ks=s,
+                vs=s, scale=0.1, left=1, right=1, sinks=0)
+
+    def call(**change):
+        a = {**good, **change}
+        return lib.b2_window_fwd(a["q"], a["k"], a["v"], a["out"], a["ws"], a["ws_bytes"], a["lengths"], a["B"], a["H"], a["Hkv"],
+                                 a["Sq"], a["Sk"], *a["qs"], *a["ks"], *a["vs"], a["scale"], a["left"], a["right"], a["sinks"], None)
+
+    assert call(B=0) == 2 and call(Sk=0) == 2 and call(Sq=-1) == 2 and call(Hkv=3) == 2
+    assert b"no multiple" in lib.b2_last_error()
+    assert call(left=-2) == 2 and call(right=-2) == 2 and call(sinks=-1) == 2
+    assert call(scale=float("nan")) == 2 and call(scale=0.0) == 2
+    assert call(k=None) == 7 and call(out=None) == 7
+    assert call(v=ODD) == 3 and call(lengths=ODD) == 3
+    assert call(ks=[1 << 20, 100, 512]) == 3 and call(vs=[1 << 20, 0, 512]) == 3 and call(qs=[1 << 20, -128, 512]) == 3
+    assert call(ks=[1 << 20, 1 << 38, 512]) == 8 and call(B=65536) == 8 and call(Sq=1 << 29) == 8
+    # single tokens of a long cache need room for their parts
+    need = ctypes.c_int64(-1)
+    assert lib.b2_window_fwd_workspace(1, 4, 4, 1, 8192, -1, 0, 0, ctypes.byref(need)) == 0 and need.value > 0
+    assert call(Sq=1, Sk=8192, left=-1, right=0, ws=FAKE, ws_bytes=need.value - 1) == 2
+    assert b"workspace" in lib.b2_last_error()
+    assert lib.b2_window_fwd_workspace(8, 24, 24, 4096, 4096, -1, 0, 0, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.b2_window_fwd_workspace(1, 4, 4, 1, 8192, -1, 0, 0, None) == 7
+    assert lib.b2_window_fwd_workspace(1, 4, 3, 1, 8192, -1, 0, 0, ctypes.byref(need)) == 2
+    x = torch.zeros((1, 2, 8, 128), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        pkg.ops.window_fwd_bhsd(x, x, x, 0.1, -1, -1)
