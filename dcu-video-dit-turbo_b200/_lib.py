@@ -69,6 +69,8 @@ ABI_VERSION = 1
 _lib = None
 _lib_path: Path | None = None
 _lib_sha256: str | None = None
+_NEVER = object()
+_lib_env: object = _NEVER   # value of B2DIT_SO for which a plain load() last answered with `_lib`
 
 
 def so_path() -> Path:
@@ -90,9 +92,13 @@ def sha256_file(path: Path) -> str:
 def load(path: str | os.PathLike | None = None):
     """Load the library (once).  Raises RuntimeError when it is missing, has the
     wrong ABI version or lacks a declared symbol: never a silent fallback."""
-    global _lib, _lib_path, _lib_sha256
+    global _lib, _lib_path, _lib_sha256, _lib_env
+    env = os.environ.get("B2DIT_SO") if path is None else _NEVER
+    if path is None and env == _lib_env:   # what every operator call meets: 1 us instead of 4 for the path
+        return _lib
     p = Path(path) if path is not None else so_path()
     if _lib is not None and _lib_path == p:
+        _lib_env = env
         return _lib
     if not p.exists():
         raise RuntimeError(
@@ -111,6 +117,7 @@ def load(path: str | os.PathLike | None = None):
     if lib.b2_version() != ABI_VERSION:
         raise RuntimeError(f"B200 DiT kernel library ABI {lib.b2_version()} != {ABI_VERSION}: {p}")
     _lib, _lib_path, _lib_sha256 = lib, p, sha256_file(p)
+    _lib_env = env
     return lib
 
 

@@ -17,6 +17,7 @@ reference project:
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -31,7 +32,9 @@ launch_count = 0
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle that torch.cuda.current_stream(t.device).cuda_stream gives, without a Stream object
+    # around it (2 us per call)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -88,7 +91,7 @@ def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> No
         stream = torch.cuda.current_stream(t.device)
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record(stream)
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         with torch.cuda.device(t.device):
             st = getattr(lib, name)(*args)
     else:
@@ -603,13 +606,18 @@ def _mx_empty(rows: int, columns: int, device):
 
 def _require_mx(q: torch.Tensor, s: torch.Tensor, what: str) -> tuple[int, int]:
     """Checks a quantised matrix (elements, scales); returns its rows and columns."""
-    _require(q.is_cuda and s.is_cuda and s.device == q.device, f"{what} and its scales must be on the same CUDA device")
-    _require(q.dtype == torch.uint8 and s.dtype == torch.uint8, f"{what} and its scales must be uint8")
-    _require(q.dim() == 2 and q.is_contiguous() and s.is_contiguous(), f"{what} must be a contiguous [M, K/2] tensor with contiguous scales")
-    m, k = q.shape[0], 2 * q.shape[1]
-    _require(k % MX_BLOCK == 0, f"{what} must have a multiple of {MX_BLOCK} columns")
-    _require(tuple(s.shape) == mxfp4_scale_shape(m, k),
-             f"the scales of {what} must have shape {mxfp4_scale_shape(m, k)}, got {tuple(s.shape)}")
+    if not (q.is_cuda and s.is_cuda and q.get_device() == s.get_device()):
+        raise RuntimeError(f"{what} and its scales must be on the same CUDA device")
+    if q.dtype != torch.uint8 or s.dtype != torch.uint8:
+        raise RuntimeError(f"{what} and its scales must be uint8")
+    if q.dim() != 2 or not q.is_contiguous() or not s.is_contiguous():
+        raise RuntimeError(f"{what} must be a contiguous [M, K/2] tensor with contiguous scales")
+    m, k = q.shape
+    k *= 2
+    if k % MX_BLOCK:
+        raise RuntimeError(f"{what} must have a multiple of {MX_BLOCK} columns")
+    if s.shape != mxfp4_scale_shape(m, k):
+        raise RuntimeError(f"the scales of {what} must have shape {mxfp4_scale_shape(m, k)}, got {tuple(s.shape)}")
     return m, k
 
 
@@ -618,8 +626,10 @@ def _quantize_mxfp4(name: str, x: torch.Tensor, halves: int):
     _require(x.is_contiguous(), "input must be contiguous")
     _require(x.dtype == torch.bfloat16, "input must be bfloat16")
     _require(x.dim() == 2, "input must be a two-dimensional tensor")
-    m, k = x.shape[0], x.shape[1] // halves
-    _require(x.shape[1] % (halves * MX_BLOCK) == 0, f"input width must be a multiple of {halves * MX_BLOCK}")
+    m, width = x.shape
+    k = width // halves
+    if width % (halves * MX_BLOCK):
+        raise RuntimeError(f"input width must be a multiple of {halves * MX_BLOCK}")
     q, s = _mx_empty(m, k, x.device)
     if m and k:
         _call(name, x, x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, _stream(x),
@@ -690,7 +700,8 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
              "x must be a contiguous CUDA bf16 [M,K] tensor")
     n, k = _require_mx(w, w_scale, "w")
     act = {None: ACT_NONE, "swiglu": ACT_SWIGLU}.get(input_act, -1)
-    _require(act >= 0, f"unknown input activation {input_act!r}")
+    if act < 0:
+        raise RuntimeError(f"unknown input activation {input_act!r}")
     _require(w.device == x.device, "all inputs must be on the same device")
     width = 2 * k if act == ACT_SWIGLU else k
     if x.shape[1] != width:
@@ -744,7 +755,7 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
     C must be a multiple of 32, at most 16384."""
     total = _rmsnorm_inputs(x, residual, weight, eps)
     m, c = x.shape
-    _require(c % MX_BLOCK == 0 and c <= 16384, f"the width must be a multiple of {MX_BLOCK}, at most 16384")
+    _require(c % MX_BLOCK == 0 and c <= 16384, "the width must be a multiple of 32, at most 16384")
     q, s = _mx_empty(m, c, x.device)
     if m:
         _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), _ptr(residual), weight.data_ptr(),
@@ -754,6 +765,14 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
 
 
 # ---- attention with a sliding window (no counterpart in the reference) --------------
+
+@functools.lru_cache(maxsize=1024)
+def _window_workspace(*sizes: int) -> int:
+    """Workspace bytes of a windowed attention call: a function of its sizes alone."""
+    need = ctypes.c_int64(0)
+    _lib.check(_lib.load().b2_window_fwd_workspace(*sizes, ctypes.byref(need)), "b2_window_fwd_workspace")
+    return need.value
+
 
 def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, left: int, right: int,
                     sinks: int = 0, kv_lengths: torch.Tensor | None = None) -> torch.Tensor:
@@ -766,18 +785,19 @@ def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     on it.  Returns the [B,H,Sq,128] transpose view of a fresh contiguous [B,Sq,H,128] tensor."""
     _require(q.is_cuda and k.is_cuda and v.is_cuda, "q, k, and v must be on a CUDA device")
     _require(q.dtype == torch.bfloat16, "kernel requires BF16 q")
-    _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, and v must have the same dtype")
+    _require(k.dtype == v.dtype == torch.bfloat16, "q, k, and v must have the same dtype")
+    _require(q.get_device() == k.get_device() == v.get_device(), "q, k, and v must be on the same CUDA device")
     _require(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, and v must use BHSD layout")
-    _require(q.device == k.device and q.device == v.device, "q, k, and v must be on the same CUDA device")
     b, h, sq, d = q.shape
-    hkv, sk = k.shape[1], k.shape[2]
-    _require(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d,
-             "k and v must have the same shape and q's batch and head dimension")
+    _, hkv, sk, _ = k.shape
+    _require(k.shape == v.shape == (b, hkv, sk, d), "k and v must have the same shape and q's batch and head dimension")
     _require(d == 128, "kernel requires head dimension 128")
     _require(b > 0 and h > 0 and sq > 0 and hkv > 0 and sk > 0, "batch, heads, and sequence lengths must be positive")
     _require(h % hkv == 0, "the query heads must be a multiple of the key heads")
-    _require(q.stride(3) == 1 and k.stride(3) == 1 and v.stride(3) == 1,
-             "q, k, and v must have contiguous last dimensions")
+    qb, qh, qs, qd = q.stride()
+    kb, kh, ks, kd = k.stride()
+    vb, vh, vs, vd = v.stride()
+    _require(qd == 1 and kd == 1 and vd == 1, "q, k, and v must have contiguous last dimensions")
     scale = float(softmax_scale)
     _require(math.isfinite(scale) and scale > 0.0, "softmax_scale must be finite and positive")
     left, right, sinks = int(left), int(right), int(sinks)
@@ -786,15 +806,14 @@ def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     left, right, sinks = min(left, sk + sq), min(right, sk + sq), min(sinks, sk)
     if kv_lengths is not None:
         _require_vector(kv_lengths, q, b, torch.int32, "kv_lengths")
-    storage = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
-    need = ctypes.c_int64(0)
-    _lib.check(_lib.load().b2_window_fwd_workspace(b, h, hkv, sq, sk, left, right, sinks, ctypes.byref(need)),
-               "b2_window_fwd_workspace")
-    workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    storage = torch.empty((b, sq, h, d), dtype=torch.bfloat16, device=q.device)
+    need = _window_workspace(b, h, hkv, sq, sk, left, right, sinks)
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     span = sk if left < 0 or right < 0 else min(sk, left + right + 1)
-    _call("b2_window_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), storage.data_ptr(), _ptr(workspace), need.value,
-          _ptr(kv_lengths), b, h, hkv, sq, sk, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], scale, left, right,
-          sinks, _stream(q), launches=2 if need.value else 1, work=("bf16", 4 * b * h * sq * span * d))
+    _call("b2_window_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), storage.data_ptr(),
+          workspace.data_ptr() if need else None, need, None if kv_lengths is None else kv_lengths.data_ptr(), b, h, hkv,
+          sq, sk, qb, qh, qs, kb, kh, ks, vb, vh, vs, scale, left, right, sinks, _stream(q),
+          launches=2 if need else 1, work=("bf16", 4 * b * h * sq * span * d))
     return storage.transpose(1, 2)
 
 
