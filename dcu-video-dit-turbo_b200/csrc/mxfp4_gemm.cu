@@ -11,6 +11,12 @@
 //   warp 1     one lane copies a stage's scales into tensor memory and issues its MMAs
 //   warps 2-5  epilogue: accumulators -> bias -> bf16 -> staging tile -> TMA store
 //
+// PAIR: two CTAs of a cluster (two SMs) make one 256 x 256 tile with cta_group::2 MMAs, each loading
+// its own 128 rows of A and its own half of W's rows (32 KB per stage and SM against 48 KB for a
+// 128 x 256 tile of one CTA): at 4 bits the tensor core eats a stage in 512 clocks, and what an SM
+// can draw from L2 in that time is what bounds the product.  The leader issues for both; W's scales
+// are needed whole in both tensor memories.  TMA loads are plain per-CTA ones.
+//
 // Tensor memory (512 columns): a tile's 256 accumulator columns, twice, leave no room for scales,
 // so the two accumulators overlap by 64 columns (0-255 and 192-447) and the scales have the last
 // 64, two stages of 24.  The epilogue reads the shared 64 columns first and then lets the next
@@ -23,6 +29,7 @@
 #include "b2_launch.h"
 #include "gemm_epilogue.cuh"
 #include "mxfp4.cuh"
+#include "sm100_pair.cuh"
 #include "sm100_ptx.cuh"
 
 namespace b2 {
@@ -45,29 +52,30 @@ constexpr int SF_COL = 448;                // scales: two buffers of 32 columns
 constexpr int SF_STRIDE = 32;
 constexpr int SFB_COL = 8;                 // within a buffer: A's 2 x 4 columns, then W's 2 x 8
 
-constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BKB;          // 16 KB
-constexpr int B_BYTES = BN * BKB;          // 32 KB
 constexpr int SFA_BYTES = 2 * kMxTileBytes;
 constexpr int SFB_BYTES = 4 * kMxTileBytes;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int SMEM_SF = STAGES * STAGE_BYTES;
 constexpr int SF_STAGE = SFA_BYTES + SFB_BYTES;
-constexpr int SMEM_OUT = SMEM_SF + STAGES * SF_STAGE;
-constexpr int SMEM_BIAS = SMEM_OUT + (EPI_THREADS / 32) * kEpiStageBytes;
-constexpr int SMEM_BARS = SMEM_BIAS + 2 * BN * 4;
-constexpr int NUM_BARS = 2 * STAGES + 2 + 1 + 2;
-constexpr int SMEM_TOTAL = 1024 + SMEM_BARS + NUM_BARS * 8 + 16;
-static_assert(SMEM_TOTAL <= 227 * 1024, "shared memory budget");
-static_assert(SMEM_OUT % 1024 == 0, "staging tiles are 1024-byte aligned");
+constexpr int SMEM_LIMIT = 227 * 1024;
+
+template <bool PAIR>
+struct Layout {
+  static constexpr int STAGES = PAIR ? 5 : 4;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;        // rows of W that one CTA loads
+  static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BKB;
+  static constexpr int SF = STAGES * STAGE_BYTES;
+  static constexpr int OUT = SF + STAGES * SF_STAGE;
+  static constexpr int BIAS = OUT + (EPI_THREADS / 32) * kEpiStageBytes;
+  static constexpr int BARS = BIAS + 2 * BN * 4;
+  static constexpr int NUM_BARS = 2 * STAGES + 2 + 1 + 2;
+  static constexpr int TOTAL = 1024 + BARS + NUM_BARS * 8 + 16;
+  static_assert(TOTAL <= SMEM_LIMIT, "shared memory budget");
+  static_assert(OUT % 1024 == 0, "staging tiles are 1024-byte aligned");
+};
 
 struct MxGemmArgs {
   int M, N, K;
   int tiles_m, tiles_n, num_tiles, k_blocks, group_m;
-  int k_tiles;                 // scale tiles along K
-  int b_row_tiles;             // scale tiles along W's rows
-  const uint8_t* a_scale;
-  const uint8_t* w_scale;
   const void* bias;
   int bias_kind;
 };
@@ -82,25 +90,55 @@ __device__ __forceinline__ void decode_tile(int tile, const MxGemmArgs& a, int& 
   n_idx = in_group / rows;
 }
 
-// contiguous global -> shared copy counted on a barrier; addresses and size multiples of 16
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
-// one scale tile: 32 lines of 16 bytes -> 32 lanes x 4 columns, repeated in all four lane quarters
+// One scale tile: 32 lines of 16 bytes -> 32 lanes x 4 columns, repeated in all four lane quarters
+// (PAIR: in each CTA, from its own shared memory).
+template <bool PAIR>
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
   // no swizzle; 8 lines of 16 bytes are contiguous, the next 8 follow 128 bytes on
   const uint64_t desc = (uint64_t)((smem_addr >> 4) & 0x3fffu) | (1ull << 16) | (8ull << 32) | (1ull << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
+#define B2_MXF4(group)                                                                                     \
+  asm volatile(                                                                                            \
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                  \
+      "tcgen05.mma.cta_group::" group                                                                      \
+      ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),          \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                              \
+      : "memory")
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (PAIR)
+    B2_MXF4("2");
+  else
+    B2_MXF4("1");
+}
+#undef B2_MXF4
+// arrive on this CTA's barrier (the leader's, when PAIR) once all its MMAs and copies so far completed
+template <bool PAIR>
+__device__ __forceinline__ void commit_here(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    tc_commit(bar);
+}
+// ... on the barrier of both CTAs, when PAIR
+template <bool PAIR>
+__device__ __forceinline__ void commit_all(uint32_t bar) {
+  if constexpr (PAIR)
+    tc_commit_pair(bar);
+  else
+    tc_commit(bar);
 }
 // Instruction descriptor of kind::mxf4: scale word halves 4-5 (W) and 29-30 (A), formats 7-9 and
 // 10-11 (1 = E2M1), N >> 3 in 17-22, scale format bit 23 (1 = E8M0), M >> 4 from bit 24.
@@ -108,15 +146,19 @@ __host__ __device__ constexpr uint32_t mx_idesc(uint32_t m, uint32_t n, uint32_t
   return ((half * 2) << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | ((half * 2) << 29);
 }
 
-__global__ void __launch_bounds__(NUM_THREADS, 1)
-mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                  const __grid_constant__ CUtensorMap tmap_out, const MxGemmArgs args) {
+template <bool PAIR>
+__device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const CUtensorMap& tmap_b,
+                                                const CUtensorMap& tmap_sa, const CUtensorMap& tmap_sb,
+                                                const CUtensorMap& tmap_out, const MxGemmArgs& args) {
+  using L = Layout<PAIR>;
+  constexpr int STAGES = L::STAGES;
+  constexpr int TILE_M = PAIR ? 2 * BM : BM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* bias_s = reinterpret_cast<float*>(smem + SMEM_BIAS);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_BARS);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
+  float* bias_s = reinterpret_cast<float*>(smem + L::BIAS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::NUM_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t ring = smem_u32(smem);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + STAGES * 8;
@@ -125,6 +167,9 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   const uint32_t sfree0 = tfree + 8;             // MMAs that read scale buffer 0 / 1 are complete
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;   // 0 = leader
+  const int first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -133,21 +178,29 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     }
     mbar_init(tfull0, 1);
     mbar_init(tfull0 + 8, 1);
-    mbar_init(tfree, EPI_THREADS / 32);
+    mbar_init(tfree, (PAIR ? 2 : 1) * EPI_THREADS / 32);
     mbar_init(sfree0, 1);
     mbar_init(sfree0 + 8, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_sa);
+    tma_prefetch_desc(&tmap_sb);
     tma_prefetch_desc(&tmap_out);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();   // both CTAs' barriers are initialised before any remote access
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -156,26 +209,32 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+      for (int tile = first_tile; ok && tile < args.num_tiles; tile += tile_step) {
         int m_idx, n_idx;
         decode_tile(tile, args, m_idx, n_idx);
-        const uint8_t* sfa = args.a_scale + (int64_t)m_idx * args.k_tiles * kMxTileBytes;
-        const uint8_t* sfb = args.w_scale + (int64_t)n_idx * 2 * args.k_tiles * kMxTileBytes;
-        const int b_tiles = min(2, args.b_row_tiles - n_idx * 2);
+        const int a_row = m_idx * TILE_M + (int)rank * BM;
+        const int b_row = n_idx * BN + (int)rank * L::B_ROWS;
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!(ok = mbar_wait(empty0 + stage * 8, phase ^ 1, abort_flag, kStatusGemmTimeout))) break;
-          const uint32_t bar = full0 + stage * 8;
-          const uint32_t dst = ring + stage * STAGE_BYTES;
-          const uint32_t sf = ring + SMEM_SF + stage * SF_STAGE;
-          // the last stage may hold one scale tile per row tile only
-          const uint32_t sf_bytes = (uint32_t)min(2, args.k_tiles - 2 * kb) * kMxTileBytes;
-          mbar_expect_tx(bar, STAGE_BYTES + (1 + b_tiles) * sf_bytes);
-          tma_load_2d(dst, &tmap_a, bar, kb * BKB, m_idx * BM);
-          tma_load_2d(dst + A_BYTES, &tmap_b, bar, kb * BKB, n_idx * BN);
-          bulk_load(sf, sfa + (int64_t)kb * 2 * kMxTileBytes, sf_bytes, bar);
-          for (int t = 0; t < b_tiles; ++t)
-            bulk_load(sf + SFA_BYTES + t * 2 * kMxTileBytes,
-                      sfb + ((int64_t)t * args.k_tiles + kb * 2) * kMxTileBytes, sf_bytes, bar);
+          const uint32_t dst = ring + stage * L::STAGE_BYTES;
+          const uint32_t sf = ring + L::SF + stage * SF_STAGE;
+          // scale tiles [row tile][k tile]: one row tile of A, two of W, two k tiles each (zeros where
+          // there are none)
+          if constexpr (PAIR) {
+            const uint32_t bar = map_to_cta(full0 + stage * 8, 0);
+            if (rank == 0) mbar_expect_tx(full0 + stage * 8, 2 * (L::STAGE_BYTES + SF_STAGE));   // both CTAs' bytes
+            tma_load_2d_pair(dst, &tmap_a, bar, kb * BKB, a_row);
+            tma_load_2d_pair(dst + A_BYTES, &tmap_b, bar, kb * BKB, b_row);
+            tma_load_3d_pair(sf, &tmap_sa, bar, 0, kb * 2, a_row / kMxTileRows);
+            tma_load_3d_pair(sf + SFA_BYTES, &tmap_sb, bar, 0, kb * 2, n_idx * (BN / kMxTileRows));
+          } else {
+            const uint32_t bar = full0 + stage * 8;
+            mbar_expect_tx(bar, L::STAGE_BYTES + SF_STAGE);
+            tma_load_2d(dst, &tmap_a, bar, kb * BKB, a_row);
+            tma_load_2d(dst + A_BYTES, &tmap_b, bar, kb * BKB, b_row);
+            tma_load_3d(sf, &tmap_sa, bar, 0, kb * 2, a_row / kMxTileRows);
+            tma_load_3d(sf + SFA_BYTES, &tmap_sb, bar, 0, kb * 2, n_idx * (BN / kMxTileRows));
+          }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -184,7 +243,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       int sbuf = 0;
@@ -192,7 +251,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       int buf = 0;
       uint32_t fphase = 0;
       bool first = true, ok = true;
-      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+      for (int tile = first_tile; ok && tile < args.num_tiles; tile += tile_step) {
         // the tile before must have left the columns that this one's accumulator shares with it
         if (!first) {
           if (!(ok = mbar_wait(tfree, fphase, abort_flag, kStatusGemmTimeout))) break;
@@ -206,22 +265,26 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           if (!(ok = mbar_wait(sfree0 + sbuf * 8, sphase ^ 1, abort_flag, kStatusGemmTimeout))) break;
           tc_fence_after();
           const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
-          const uint32_t sf = ring + SMEM_SF + stage * SF_STAGE;
+          const uint32_t sf = ring + L::SF + stage * SF_STAGE;
           const uint32_t sf_tmem = tmem_base + SF_COL + sbuf * SF_STRIDE;
           // [k tile][row group of 32]: 4 columns of A per k tile, 8 of W
-          for (int kt = 0; kt * 2 < steps; ++kt) {
-            scales_to_tmem(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            scales_to_tmem<PAIR>(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
+#pragma unroll
             for (int t = 0; t < 2; ++t)
-              scales_to_tmem(sf_tmem + SFB_COL + kt * 8 + t * 4, sf + SFA_BYTES + (t * 2 + kt) * kMxTileBytes);
+              scales_to_tmem<PAIR>(sf_tmem + SFB_COL + kt * 8 + t * 4, sf + SFA_BYTES + (t * 2 + kt) * kMxTileBytes);
           }
-          const uint32_t a_addr = ring + stage * STAGE_BYTES;
+          const uint32_t a_addr = ring + stage * L::STAGE_BYTES;
           const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
           const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
-          for (int k = 0; k < steps; ++k)
-            mma_mxf4(d_tmem, adesc + 2 * k, bdesc + 2 * k, (k & 1) ? mx_idesc(BM, BN, 1) : mx_idesc(BM, BN, 0),
-                     sf_tmem + (k >> 1) * 4, sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
-          tc_commit(sfree0 + sbuf * 8);
-          tc_commit(empty0 + stage * 8);
+#pragma unroll
+          for (int k = 0; k < BKE / UMMA_K; ++k)
+            if (k < steps)
+              mma_mxf4<PAIR>(d_tmem, adesc + 2 * k, bdesc + 2 * k, mx_idesc(TILE_M, BN, k & 1), sf_tmem + (k >> 1) * 4,
+                             sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
+          commit_here<PAIR>(sfree0 + sbuf * 8);
+          commit_all<PAIR>(empty0 + stage * 8);
           sbuf ^= 1;
           if (sbuf == 0) sphase ^= 1;
           if (++stage == STAGES) {
@@ -230,7 +293,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           }
         }
         if (!ok) break;
-        tc_commit(tfull0 + buf * 8);
+        commit_all<PAIR>(tfull0 + buf * 8);
         buf ^= 1;
       }
     }
@@ -239,12 +302,13 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     const int et = threadIdx.x - 64;
     int buf = 0;
     uint32_t buf_phase = 0;
-    const uint32_t stage = ring + SMEM_OUT + quarter * kEpiStageBytes;
-    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
+    const uint32_t stage = ring + L::OUT + quarter * kEpiStageBytes;
+    const uint32_t tfree_leader = PAIR ? map_to_cta(tfree, 0) : tfree;
+    for (int tile = first_tile; tile < args.num_tiles; tile += tile_step) {
       int m_idx, n_idx;
       decode_tile(tile, args, m_idx, n_idx);
       const int col0 = n_idx * BN;
-      const int row_warp = m_idx * BM + quarter * 32;
+      const int row_warp = m_idx * TILE_M + (int)rank * BM + quarter * 32;
       float* bias = bias_s + buf * BN;
       for (int c = et; c < BN; c += EPI_THREADS) {
         float b = 0.f;
@@ -270,7 +334,12 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         if (i == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tfree);
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_cluster(tfree_leader);
+            else
+              mbar_arrive(tfree);
+          }
         }
         if (col0 + c >= args.N) continue;
         if (lane == 0) bulk_wait_group_read<0>();   // the previous store has read the tile
@@ -305,10 +374,28 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();   // neither CTA retires (or frees tensor memory) before both are done
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else
+      tmem_dealloc(tmem_base, TMEM_COLS);
   }
+}
+
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                  const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
+                  const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmArgs args) {
+  mxfp4_gemm_body<false>(tmap_a, tmap_b, tmap_sa, tmap_sb, tmap_out, args);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+mxfp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                       const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
+                       const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmArgs args) {
+  mxfp4_gemm_body<true>(tmap_a, tmap_b, tmap_sa, tmap_sb, tmap_out, args);
 }
 
 int encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int box_rows) {
@@ -322,6 +409,22 @@ int encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: tensor map encode failed (%d)", (int)r);
+  return B2_OK;
+}
+
+// Scale bytes as [row tile][k tile][128 words]; a box is two k tiles of `row_tiles` row tiles.
+int encode_scales(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int row_tiles) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t k_tiles = (cuuint64_t)((k + kMxTileCols - 1) / kMxTileCols);
+  const cuuint64_t dims[3] = {kMxTileBytes / 4, k_tiles, (cuuint64_t)((rows + kMxTileRows - 1) / kMxTileRows)};
+  const cuuint64_t strides[2] = {kMxTileBytes, kMxTileBytes * k_tiles};
+  const cuuint32_t box[3] = {kMxTileBytes / 4, 2, (cuuint32_t)row_tiles};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: scale tensor map encode failed (%d)", (int)r);
   return B2_OK;
 }
 
@@ -344,20 +447,45 @@ int encode_out(CUtensorMap* map, void* base, int64_t M, int64_t N) {
 int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W, const uint8_t* w_scale,
                       const void* bias, int bias_kind, void* out, int64_t M, int64_t N, int64_t K,
                       cudaStream_t stream) {
+  // slot.a = SMs, slot.b = CTA pairs that run at once (0: none)
   static PerDeviceSetup per_device;
   const DeviceSlot* slot = nullptr;
   const int setup_status = per_device.get("mxfp4_gemm", [](int dev, DeviceSlot& s) -> int {
-    cudaError_t e = cudaFuncSetAttribute(mxfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(mxfp4_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Layout<false>::TOTAL);
+    if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
+    e = cudaFuncSetAttribute(mxfp4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<true>::TOTAL);
     if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
     s.a = kNumSMsB200;
     cudaDeviceGetAttribute(&s.a, cudaDevAttrMultiProcessorCount, dev);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(s.a / 2 * 2));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = Layout<true>::TOTAL;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&s.b, mxfp4_gemm_pair_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      s.b = 0;
+    }
     return B2_OK;
   }, &slot);
   if (setup_status != B2_OK) return setup_status;
-  CUtensorMap ta, tb, tout;
+  const bool pair = slot->b > 0 && M > BM;
+  const int tile_m = pair ? 2 * BM : BM;
+  CUtensorMap ta, tb, tsa, tsb, tout;
   int st = encode_operand(&ta, A, M, K, BM);
   if (st != B2_OK) return st;
-  st = encode_operand(&tb, W, N, K, BN);
+  st = encode_operand(&tb, W, N, K, pair ? Layout<true>::B_ROWS : Layout<false>::B_ROWS);
+  if (st != B2_OK) return st;
+  st = encode_scales(&tsa, a_scale, M, K, 1);
+  if (st != B2_OK) return st;
+  st = encode_scales(&tsb, w_scale, N, K, BN / kMxTileRows);
   if (st != B2_OK) return st;
   st = encode_out(&tout, out, M, N);
   if (st != B2_OK) return st;
@@ -365,21 +493,22 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
   a.M = (int)M;
   a.N = (int)N;
   a.K = (int)K;
-  a.tiles_m = (int)((M + BM - 1) / BM);
+  a.tiles_m = (int)((M + tile_m - 1) / tile_m);
   a.tiles_n = (int)((N + BN - 1) / BN);
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > 0x7fffffffLL) return fail(B2_TOO_LARGE, "mxfp4_gemm: too many tiles");
   a.num_tiles = (int)tiles;
   a.k_blocks = (int)((K + BKE - 1) / BKE);
-  a.group_m = 16;
-  a.k_tiles = (int)((K + kMxTileCols - 1) / kMxTileCols);
-  a.b_row_tiles = (int)((N + kMxTileRows - 1) / kMxTileRows);
-  a.a_scale = a_scale;
-  a.w_scale = w_scale;
+  a.group_m = pair ? 8 : 16;
   a.bias = bias;
   a.bias_kind = bias_kind;
-  const int grid = a.num_tiles < slot->a ? a.num_tiles : slot->a;
-  mxfp4_gemm_kernel<<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(ta, tb, tout, a);
+  if (pair) {
+    const int clusters = a.num_tiles < slot->b ? a.num_tiles : slot->b;
+    mxfp4_gemm_pair_kernel<<<clusters * 2, NUM_THREADS, Layout<true>::TOTAL, stream>>>(ta, tb, tsa, tsb, tout, a);
+  } else {
+    const int grid = a.num_tiles < slot->a ? a.num_tiles : slot->a;
+    mxfp4_gemm_kernel<<<grid, NUM_THREADS, Layout<false>::TOTAL, stream>>>(ta, tb, tsa, tsb, tout, a);
+  }
   return check_launch("mxfp4_gemm");
 }
 
