@@ -67,7 +67,7 @@ struct Layout {
   static constexpr int OUT = SF + STAGES * SF_STAGE;
   static constexpr int BIAS = OUT + (EPI_THREADS / 32) * kEpiStageBytes;
   static constexpr int BARS = BIAS + 2 * BN * 4;
-  static constexpr int NUM_BARS = 2 * STAGES + 2 + 1 + 2;
+  static constexpr int NUM_BARS = 2 * STAGES + 2 + 1;
   static constexpr int TOTAL = 1024 + BARS + NUM_BARS * 8 + 16;
   static_assert(TOTAL <= SMEM_LIMIT, "shared memory budget");
   static_assert(OUT % 1024 == 0, "staging tiles are 1024-byte aligned");
@@ -124,15 +124,7 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64
     B2_MXF4("1");
 }
 #undef B2_MXF4
-// arrive on this CTA's barrier (the leader's, when PAIR) once all its MMAs and copies so far completed
-template <bool PAIR>
-__device__ __forceinline__ void commit_here(uint32_t bar) {
-  if constexpr (PAIR)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-  else
-    tc_commit(bar);
-}
-// ... on the barrier of both CTAs, when PAIR
+// Arrive on the CTA's barrier (on both CTAs' when PAIR) once all MMAs and copies so far completed.
 template <bool PAIR>
 __device__ __forceinline__ void commit_all(uint32_t bar) {
   if constexpr (PAIR)
@@ -164,7 +156,6 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + STAGES * 8;
   const uint32_t tfull0 = empty0 + STAGES * 8;   // accumulator complete (2)
   const uint32_t tfree = tfull0 + 2 * 8;         // the shared columns of the tile before are read
-  const uint32_t sfree0 = tfree + 8;             // MMAs that read scale buffer 0 / 1 are complete
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;   // 0 = leader
@@ -179,8 +170,6 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
     mbar_init(tfull0, 1);
     mbar_init(tfull0 + 8, 1);
     mbar_init(tfree, (PAIR ? 2 : 1) * EPI_THREADS / 32);
-    mbar_init(sfree0, 1);
-    mbar_init(sfree0 + 8, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmap_a);
@@ -243,14 +232,18 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
+      // The whole warp walks the loop and one elected lane issues: without a lane-divergent region
+      // around them, addresses and descriptors stay warp-uniform.
+      const bool leader = elect_one() != 0;
       int stage = 0;
       uint32_t phase = 0;
       int sbuf = 0;
-      uint32_t sphase = 0;
       int buf = 0;
       uint32_t fphase = 0;
       bool first = true, ok = true;
+      int back = STAGES - 2;   // ring position of two stages ago, and the parity of its release
+      uint32_t back_phase = 1;
       for (int tile = first_tile; ok && tile < args.num_tiles; tile += tile_step) {
         // the tile before must have left the columns that this one's accumulator shares with it
         if (!first) {
@@ -261,39 +254,44 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
         first = false;
         const uint32_t d_tmem = tmem_base + (buf ? ACC1 : 0);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
+          // the stage is filled, and the MMAs that used this scale buffer (two stages ago) are done
           if (!(ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout))) break;
-          if (!(ok = mbar_wait(sfree0 + sbuf * 8, sphase ^ 1, abort_flag, kStatusGemmTimeout))) break;
+          if (!(ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout))) break;
           tc_fence_after();
           const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
           const uint32_t sf = ring + L::SF + stage * SF_STAGE;
           const uint32_t sf_tmem = tmem_base + SF_COL + sbuf * SF_STRIDE;
-          // [k tile][row group of 32]: 4 columns of A per k tile, 8 of W
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            scales_to_tmem<PAIR>(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-              scales_to_tmem<PAIR>(sf_tmem + SFB_COL + kt * 8 + t * 4, sf + SFA_BYTES + (t * 2 + kt) * kMxTileBytes);
-          }
           const uint32_t a_addr = ring + stage * L::STAGE_BYTES;
           const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
           const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
+          if (leader) {
+            // [k tile][row group of 32]: 4 columns of A per k tile, 8 of W
 #pragma unroll
-          for (int k = 0; k < BKE / UMMA_K; ++k)
-            if (k < steps)
-              mma_mxf4<PAIR>(d_tmem, adesc + 2 * k, bdesc + 2 * k, mx_idesc(TILE_M, BN, k & 1), sf_tmem + (k >> 1) * 4,
-                             sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
-          commit_here<PAIR>(sfree0 + sbuf * 8);
-          commit_all<PAIR>(empty0 + stage * 8);
+            for (int kt = 0; kt < 2; ++kt) {
+              scales_to_tmem<PAIR>(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+                scales_to_tmem<PAIR>(sf_tmem + SFB_COL + kt * 8 + t * 4, sf + SFA_BYTES + (t * 2 + kt) * kMxTileBytes);
+            }
+#pragma unroll
+            for (int k = 0; k < BKE / UMMA_K; ++k)
+              if (k < steps)
+                mma_mxf4<PAIR>(d_tmem, adesc + 2 * k, bdesc + 2 * k, mx_idesc(TILE_M, BN, k & 1), sf_tmem + (k >> 1) * 4,
+                               sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
+            commit_all<PAIR>(empty0 + stage * 8);
+          }
           sbuf ^= 1;
-          if (sbuf == 0) sphase ^= 1;
+          if (++back == STAGES) {
+            back = 0;
+            back_phase ^= 1;
+          }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        commit_all<PAIR>(tfull0 + buf * 8);
+        if (leader) commit_all<PAIR>(tfull0 + buf * 8);
         buf ^= 1;
       }
     }
