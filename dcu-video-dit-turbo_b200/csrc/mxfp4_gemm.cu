@@ -24,6 +24,10 @@
 // a whole epilogue.  A stage's scales may replace those of two stages before only when that stage's
 // MMAs are complete (their commit is waited for): the order of an MMA and a later copy into its
 // scales is not promised.
+// Calls whose 128 x 128 tiles do not fill the GPU once (few rows, above all) are bound by how many SMs
+// pull on the weights: mxfp4_gemm_split_kernel gives each such tile to a cluster of 1, 2, 4 or 8
+// CTAs that take a share of K each; their fp32 sums meet in shared memory, where every CTA adds up
+// its share of the columns (in rank order: the same bits every time) and stores it.
 // Every wait is bounded; on a timeout the kernel records a status word and returns.
 #include "b2_common.cuh"
 #include "b2_launch.h"
@@ -396,6 +400,196 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   mxfp4_gemm_body<true>(tmap_a, tmap_b, tmap_sa, tmap_sb, tmap_out, args);
 }
 
+// ---- few tiles: a cluster of CTAs shares K ----------------------------------------------------
+
+constexpr int SBN = 128;                   // columns per tile
+constexpr int S_STAGES = 5;
+constexpr int S_STAGE_BYTES = A_BYTES + SBN * BKB;
+constexpr int S_SF_STAGE = 4 * kMxTileBytes;             // two k tiles of A, two of W
+constexpr int S_SF = S_STAGES * S_STAGE_BYTES;
+constexpr int S_BARS = S_SF + S_STAGES * S_SF_STAGE;
+constexpr int S_NUM_BARS = 2 * S_STAGES + 1;
+constexpr int S_TOTAL = 1024 + S_BARS + S_NUM_BARS * 8 + 16;
+constexpr int S_TMEM_COLS = 256;           // 128 of accumulator, scales from column 128: two buffers of 16 in 32
+constexpr int S_SF_COL = 128;
+constexpr int S_PITCH = SBN + 4;           // floats per row of a CTA's sums: rows start 4 banks apart
+static_assert(BM * S_PITCH * 4 <= S_SF, "the sums take the place of the operand ring");
+static_assert(S_TOTAL <= SMEM_LIMIT, "shared memory budget");
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                        const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
+                        __nv_bfloat16* __restrict__ out, int splits, const __grid_constant__ MxGemmArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S_NUM_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + S_STAGES * 8, tfull = empty0 + S_STAGES * 8;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const int m_idx = tile % args.tiles_m, n_idx = tile / args.tiles_m;
+  const int kb0 = (int)((int64_t)args.k_blocks * rank / splits);
+  const int kb1 = (int)((int64_t)args.k_blocks * (rank + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S_NUM_BARS; ++i) mbar_init(full0 + i * 8, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_sa);
+    tma_prefetch_desc(&tmap_sb);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), S_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(empty0 + stage * 8, phase ^ 1, abort_flag, kStatusGemmTimeout)) break;
+        const uint32_t bar = full0 + stage * 8;
+        const uint32_t dst = ring + stage * S_STAGE_BYTES;
+        const uint32_t sf = ring + S_SF + stage * S_SF_STAGE;
+        mbar_expect_tx(bar, S_STAGE_BYTES + S_SF_STAGE);
+        tma_load_2d(dst + A_BYTES, &tmap_b, bar, kb * BKB, n_idx * SBN);
+        tma_load_3d(sf + SFA_BYTES, &tmap_sb, bar, 0, kb * 2, n_idx);
+        tma_load_2d(dst, &tmap_a, bar, kb * BKB, m_idx * BM);
+        tma_load_3d(sf, &tmap_sa, bar, 0, kb * 2, m_idx);
+        if (++stage == S_STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one() != 0;
+    int stage = 0, sbuf = 0;
+    uint32_t phase = 0;
+    int back = S_STAGES - 2;
+    uint32_t back_phase = 1;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!(ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout))) break;
+      if (!(ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout))) break;
+      tc_fence_after();
+      const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
+      const uint32_t sf = ring + S_SF + stage * S_SF_STAGE;
+      const uint32_t sf_tmem = tmem_base + S_SF_COL + sbuf * SF_STRIDE;
+      const uint32_t a_addr = ring + stage * S_STAGE_BYTES;
+      const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
+      const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
+      if (leader) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          scales_to_tmem<false>(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
+          scales_to_tmem<false>(sf_tmem + SFB_COL + kt * 4, sf + SFA_BYTES + kt * kMxTileBytes);
+        }
+#pragma unroll
+        for (int k = 0; k < BKE / UMMA_K; ++k)
+          if (k < steps)
+            mma_mxf4<false>(tmem_base, adesc + 2 * k, bdesc + 2 * k, mx_idesc(BM, SBN, k & 1), sf_tmem + (k >> 1) * 4,
+                            sf_tmem + SFB_COL + (k >> 1) * 4, (kb > kb0 || k > 0) ? 1u : 0u);
+        tc_commit(empty0 + stage * 8);
+      }
+      sbuf ^= 1;
+      if (++back == S_STAGES) {
+        back = 0;
+        back_phase ^= 1;
+      }
+      if (++stage == S_STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (ok && leader) tc_commit(tfull);
+  } else {
+    // every MMA is complete and every load has been used: the sums go where the ring was
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    if (mbar_wait(tfull, 0, abort_flag, kStatusGemmTimeout) && m_idx * BM + quarter * 32 < args.M) {
+      tc_fence_after();
+      float* dst = reinterpret_cast<float*>(smem) + row * S_PITCH;
+#pragma unroll 1
+      for (int c = 0; c < SBN; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem_base + c + ((uint32_t)(quarter * 32) << 16), v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(dst + c)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  if (splits > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  // this CTA's share of the columns, eight per thread and step
+  const int share = SBN / splits;
+  const int groups = share / 8;
+  const int rows = min(BM, args.M - m_idx * BM);
+  if (*abort_flag == 0) {
+    for (int i = threadIdx.x; i < rows * groups; i += NUM_THREADS) {
+      const int row = i / groups;
+      const int c = rank * share + (i - row * groups) * 8;
+      const int col = n_idx * SBN + c;
+      if (col >= args.N) continue;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = 0.f;
+        if (args.bias_kind == B2_BIAS_BF16) f[j] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(args.bias)[col + j]);
+        if (args.bias_kind == B2_BIAS_FP32) f[j] = reinterpret_cast<const float*>(args.bias)[col + j];
+      }
+      const uint32_t at = ring + (row * S_PITCH + c) * 4;
+      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+      for (int r = 0; r < splits; ++r) {
+        const uint32_t src = splits > 1 ? map_to_cta(at, r) : at;
+        const float4 x = ld_cluster_f4(src), y = ld_cluster_f4(src + 16);
+        lo = make_float4(lo.x + x.x, lo.y + x.y, lo.z + x.z, lo.w + x.w);
+        hi = make_float4(hi.x + y.x, hi.y + y.y, hi.z + y.z, hi.w + y.w);
+      }
+      uint4 o;
+      o.x = pack_bf16x2_rn(lo.x + f[0], lo.y + f[1]);
+      o.y = pack_bf16x2_rn(lo.z + f[2], lo.w + f[3]);
+      o.z = pack_bf16x2_rn(hi.x + f[4], hi.y + f[5]);
+      o.w = pack_bf16x2_rn(hi.z + f[6], hi.w + f[7]);
+      *reinterpret_cast<uint4*>(out + (int64_t)(m_idx * BM + row) * args.N + col) = o;
+    }
+  } else {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 200000) {
+    }
+  }
+  if (splits > 1)
+    cluster_sync_all();   // no CTA retires while another reads its sums
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S_TMEM_COLS);
+  }
+}
+
 int encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int box_rows) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: cuTensorMapEncodeTiled is unavailable");
@@ -454,6 +648,8 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
     if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
     e = cudaFuncSetAttribute(mxfp4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<true>::TOTAL);
     if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
+    e = cudaFuncSetAttribute(mxfp4_gemm_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_TOTAL);
+    if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: smem attribute: %s", cudaGetErrorString(e));
     s.a = kNumSMsB200;
     cudaDeviceGetAttribute(&s.a, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchConfig_t cfg = {};
@@ -474,9 +670,49 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
     return B2_OK;
   }, &slot);
   if (setup_status != B2_OK) return setup_status;
+  CUtensorMap ta, tb, tsa, tsb, tout;
+  MxGemmArgs a;
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.k_blocks = (int)((K + BKE - 1) / BKE);
+  a.bias = bias;
+  a.bias_kind = bias_kind;
+  a.group_m = 1;
+  // one 128 x 128 tile (or a share of its K) per SM, while there are SMs
+  const int64_t small_tiles = ((M + BM - 1) / BM) * ((N + SBN - 1) / SBN);
+  if (small_tiles <= slot->a) {
+    int splits = 1;
+    while (splits < 8 && small_tiles * splits * 2 <= slot->a && splits * 2 <= a.k_blocks) splits *= 2;
+    int st = encode_operand(&ta, A, M, K, BM);
+    if (st == B2_OK) st = encode_operand(&tb, W, N, K, SBN);
+    if (st == B2_OK) st = encode_scales(&tsa, a_scale, M, K, 1);
+    if (st == B2_OK) st = encode_scales(&tsb, w_scale, N, K, 1);
+    if (st != B2_OK) return st;
+    a.tiles_m = (int)((M + BM - 1) / BM);
+    a.tiles_n = (int)((N + SBN - 1) / SBN);
+    a.num_tiles = (int)small_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(small_tiles * splits));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = S_TOTAL;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)splits;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, mxfp4_gemm_split_kernel, ta, tb, tsa, tsb, (__nv_bfloat16*)out, splits, a);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(B2_LAUNCH_FAILED, "mxfp4_gemm: launch failed: %s", cudaGetErrorString(e));
+    }
+    return B2_OK;
+  }
   const bool pair = slot->b > 0 && M > BM;
   const int tile_m = pair ? 2 * BM : BM;
-  CUtensorMap ta, tb, tsa, tsb, tout;
   int st = encode_operand(&ta, A, M, K, BM);
   if (st != B2_OK) return st;
   st = encode_operand(&tb, W, N, K, pair ? Layout<true>::B_ROWS : Layout<false>::B_ROWS);
@@ -487,19 +723,12 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
   if (st != B2_OK) return st;
   st = encode_out(&tout, out, M, N);
   if (st != B2_OK) return st;
-  MxGemmArgs a;
-  a.M = (int)M;
-  a.N = (int)N;
-  a.K = (int)K;
   a.tiles_m = (int)((M + tile_m - 1) / tile_m);
   a.tiles_n = (int)((N + BN - 1) / BN);
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > 0x7fffffffLL) return fail(B2_TOO_LARGE, "mxfp4_gemm: too many tiles");
   a.num_tiles = (int)tiles;
-  a.k_blocks = (int)((K + BKE - 1) / BKE);
   a.group_m = pair ? 8 : 16;
-  a.bias = bias;
-  a.bias_kind = bias_kind;
   if (pair) {
     const int clusters = a.num_tiles < slot->b ? a.num_tiles : slot->b;
     mxfp4_gemm_pair_kernel<<<clusters * 2, NUM_THREADS, Layout<true>::TOTAL, stream>>>(ta, tb, tsa, tsb, tout, a);
