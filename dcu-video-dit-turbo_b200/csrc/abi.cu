@@ -67,7 +67,8 @@ int b2_check_device_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "stream synchronize: %s", cudaGetErrorString(e));
   const unsigned int word = read_clear_status_gemm() | read_clear_status_gemm2() | read_clear_status_flash() |
-                            read_clear_status_flash2() | read_clear_status_mxfp4() | read_clear_status_window();
+                            read_clear_status_flash2() | read_clear_status_mxfp4() |
+                            read_clear_status_mxfp4_quantize() | read_clear_status_window();
   if (word == 0xffffffffu) return fail(B2_LAUNCH_FAILED, "status word could not be read");
   if (word != 0) return fail(B2_TIMEOUT, "device-side bounded wait gave up (code 0x%x)", word);
   return B2_OK;

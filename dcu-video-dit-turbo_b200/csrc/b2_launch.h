@@ -86,6 +86,7 @@ unsigned int read_clear_status_gemm2();
 unsigned int read_clear_status_flash();
 unsigned int read_clear_status_flash2();
 unsigned int read_clear_status_mxfp4();
+unsigned int read_clear_status_mxfp4_quantize();
 unsigned int read_clear_status_window();
 
 }  // namespace b2

@@ -79,15 +79,37 @@ __device__ __forceinline__ uint32_t mx_absmax_bits(uint32_t acc, uint32_t w) {
   return __vmaxu2(acc, w & 0x7fff7fffu);
 }
 
+// The larger exponent field of eight fp32 values, as packed halves: the upper halves hold it, and
+// the order of those (sign dropped) is the order of the values.
+__device__ __forceinline__ uint32_t mx_absmax_halves(const float (&f)[8]) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __byte_perm(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]), 0x7632) & 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(h[0], h[1]), __vmaxu2(h[2], h[3]));
+}
+// Scale byte of a block from the packed halves of its four lanes (neighbours).
+__device__ __forceinline__ uint32_t mx_block_byte(uint32_t halves) {
+  halves = __vmaxu2(halves, __shfl_xor_sync(0xffffffffu, halves, 1));
+  halves = __vmaxu2(halves, __shfl_xor_sync(0xffffffffu, halves, 2));
+  return mx_scale_byte(max(halves & 0xffffu, halves >> 16) >> 7);
+}
 // The four blocks' bytes of one row's column tile, from the 16 consecutive lanes that hold its 128
 // columns (four lanes per block, all with their block's byte): the word in every lane.
-__device__ __forceinline__ uint32_t mx_gather_word(uint32_t byte, uint32_t lane_mask) {
-  const int base = threadIdx.x & 16;
-  uint32_t w = __shfl_sync(lane_mask, byte, base);
-  w |= __shfl_sync(lane_mask, byte, base + 4) << 8;
-  w |= __shfl_sync(lane_mask, byte, base + 8) << 16;
-  w |= __shfl_sync(lane_mask, byte, base + 12) << 24;
+__device__ __forceinline__ uint32_t mx_gather_word(uint32_t byte) {
+  uint32_t w = byte << ((threadIdx.x & 12) * 2);
+  w |= __shfl_xor_sync(0xffffffffu, w, 4);
+  w |= __shfl_xor_sync(0xffffffffu, w, 8);
   return w;
+}
+// The packed elements of a lane's eight columns under their block's byte.
+__device__ __forceinline__ uint32_t mx_quantize8(const float (&f)[8], uint32_t byte) {
+  const float inv = mx_inverse_scale(byte);
+  const uint64_t inv2 = pack2(inv, inv);
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(mul2(pack2(f[2 * i], f[2 * i + 1]), inv2), s[2 * i], s[2 * i + 1]);
+  return byte == 255u ? 0u : mx_pack8(s);
 }
 
 }  // namespace b2

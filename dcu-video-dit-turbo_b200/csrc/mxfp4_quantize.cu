@@ -2,104 +2,152 @@
 // the values of rowwise int8.
 //
 // All are bound by memory: quantising K columns of a row moves 2K (4K with SwiGLU) bytes in and
-// K/2 + K/32 out.  One CTA takes one scale tile, 128 rows x 128 columns: 16 lanes hold a row's 128
-// columns, one 16-byte load each (four lanes per block of 32, so the block's maximum is two
-// shuffles), and a thread's eight rows are loaded before the first is used.  The tile's 512 scale
-// bytes meet in shared memory and leave as full lines; written row by row they would be 4-byte
-// pieces of eight lines each.
+// K/2 + K/32 out.  The unit is one scale tile, 128 rows x 128 columns: 16 lanes hold a row's 128
+// columns, 16 bytes each (four lanes per block of 32, so the block's maximum is two shuffles).  The
+// tile's 512 scale bytes meet in shared memory and leave as full lines; written row by row they
+// would be 4-byte pieces of eight lines each.
 #include "b2_common.cuh"
 #include "b2_launch.h"
 #include "mxfp4.cuh"
+#include "sm100_ptx.cuh"
 
 namespace b2 {
+
+unsigned int read_clear_status_mxfp4_quantize() { return read_and_clear_device_status(); }
+
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRowsPerPass = kThreads / 16;                 // 16
 constexpr int kPasses = kMxTileRows / kRowsPerPass;         // 8
 
-// silu(g) * u in fp32: g / (1 + exp(-g)); the exponential and the reciprocal are the fast ones (a
-// few units in the last place of fp32), five decimal digits below the step of the 4-bit elements.
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  const float e = __expf(-g);
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+// silu(g) * u = g / (1 + 2^(-g log2 e)) * u of a pair, in fp32 with the fast exponential and
+// reciprocal (a few units in the last place, five decimal digits below the step of the 4-bit
+// elements).  Below about -87 the reciprocal is flushed to zero: products under 1e-36 vanish.
+__device__ __forceinline__ uint64_t silu_mul2(uint64_t g, uint64_t u) {
+  float x0, x1;
+  unpack2(mul2(g, pack2(-1.4426950408889634f, -1.4426950408889634f)), x0, x1);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x1));
+  unpack2(add2(pack2(x0, x1), pack2(1.0f, 1.0f)), x0, x1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x1));
+  return mul2(mul2(g, pack2(x0, x1)), u);
 }
 
-// 8 fp32 of each of 4 neighbouring lanes make a block: its packed elements (returned) and byte.
-__device__ __forceinline__ uint32_t quantize8(const float (&f)[8], uint32_t absmax_bits, uint32_t& byte) {
-  byte = mx_scale_byte(absmax_bits >> 23);
-  const float inv = mx_inverse_scale(byte);
-  float s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = f[i] * inv;
-  return byte == 255u ? 0u : mx_pack8(s);
-}
+// A stage is 32 KB: a whole tile's rows, or with SwiGLU half of them, gate and up.
+constexpr int kStages = 3;
+constexpr int kBoxBytes = 64 * kMxTileCols * 2;             // 64 rows x 128 columns
+constexpr int kStageBytes = 2 * kBoxBytes;
+constexpr int kTileBuf = kStages * kStageBytes;             // scale bytes of the tile in hand, twice
+constexpr int kBarOffset = kTileBuf + 2 * kMxTileBytes;
+constexpr int kQuantSmem = 128 + kBarOffset + 2 * kStages * 8 + 16;
 
+// Persistent: two CTAs per SM walk the tiles, one more warp keeps the ring of TMA loads full, so what
+// is in flight does not depend on how many loads the compiler keeps together (a thread per 16-byte
+// load and row took 154 us for 109099 x 3072 and 293 us with SwiGLU).  Rows and columns outside
+// the matrix arrive as zeros.
 template <bool SWIGLU>
-__global__ void __launch_bounds__(kThreads)
-quantize_mxfp4_kernel(const uint4* __restrict__ x, uint32_t* __restrict__ q, uint8_t* __restrict__ scales,
-                      int M, int K, int col_tiles) {
-  __shared__ uint32_t tile[kMxTileBytes / 4];
-  const int ct = blockIdx.x % col_tiles;
-  const int rt = blockIdx.x / col_tiles;
-  const int lane16 = threadIdx.x & 15;
-  const int row_in_pass = threadIdx.x >> 4;
-  const int col = ct * kMxTileCols + lane16 * 8;
-  const bool col_ok = col < K;                              // K % 32 == 0: a block is in or out whole
-  const int64_t row_vec = (SWIGLU ? 2 : 1) * (int64_t)(K / 8);
-  uint4 v[kPasses], u[SWIGLU ? kPasses : 1];
-#pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int row = rt * kMxTileRows + p * kRowsPerPass + row_in_pass;
-    const bool live = col_ok && row < M;
-    const uint4* src = x + (int64_t)row * row_vec + col / 8;
-    v[p] = live ? ldg_stream(src) : make_uint4(0, 0, 0, 0);
-    if constexpr (SWIGLU) u[p] = live ? ldg_stream(src + K / 8) : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int r = p * kRowsPerPass + row_in_pass;
-    const int row = rt * kMxTileRows + r;
-    const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = bf16lo_to_f32(w[i]);
-      f[2 * i + 1] = bf16hi_to_f32(w[i]);
+__global__ void __launch_bounds__(kThreads + 32, 2)
+quantize_mxfp4_kernel(const __grid_constant__ CUtensorMap tmap, uint32_t* __restrict__ q, uint8_t* __restrict__ scales,
+                      int M, int K, int col_tiles, int tiles) {
+  constexpr int PARTS = SWIGLU ? 2 : 1;                     // stages per tile
+  constexpr int PART_PASSES = kPasses / PARTS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  const uint32_t full0 = smem_u32(smem + kBarOffset), empty0 = full0 + kStages * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kBarOffset + 2 * kStages * 8);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full0 + i * 8, 1);
+      mbar_init(empty0 + i * 8, kThreads / 32);
     }
-    uint32_t m;
-    if constexpr (SWIGLU) {
-      const uint32_t uw[4] = {u[p].x, u[p].y, u[p].z, u[p].w};
-      m = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = silu_mul(f[2 * i], bf16lo_to_f32(uw[i]));
-        f[2 * i + 1] = silu_mul(f[2 * i + 1], bf16hi_to_f32(uw[i]));
-        m = max(m, max(__float_as_uint(f[2 * i]) & 0x7fffffffu, __float_as_uint(f[2 * i + 1]) & 0x7fffffffu));
-      }
-    } else {
-      m = mx_absmax_bits(mx_absmax_bits(mx_absmax_bits(w[0] & 0x7fff7fffu, w[1]), w[2]), w[3]);
-      m = max(m << 16, m & 0xffff0000u);                    // the larger half, as fp32 bits
-    }
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    uint32_t byte;
-    const uint32_t packed = quantize8(f, m, byte);
-    if (col_ok && row < M) q[(int64_t)row * (K / 8) + col / 8] = packed;
-    const uint32_t word = mx_gather_word(byte, 0xffffffffu);   // rows and blocks outside hold zeros: byte 0
-    if (lane16 == 0) tile[mx_scale_offset(r, 0) / 4] = word;
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap);
   }
   __syncthreads();
-  if (threadIdx.x < kMxTileBytes / 16)
-    reinterpret_cast<uint4*>(scales + (int64_t)blockIdx.x * kMxTileBytes)[threadIdx.x] =
-        reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&]() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  };
+  if (threadIdx.x >= kThreads) {
+    if (threadIdx.x == kThreads) {
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const int col = (t % col_tiles) * kMxTileCols, row = (t / col_tiles) * kMxTileRows;
+        for (int part = 0; part < PARTS; ++part) {
+          if (!(ok = mbar_wait(empty0 + stage * 8, phase ^ 1, abort_flag, kStatusGemmTimeout))) break;
+          const uint32_t dst = smem_u32(smem + stage * kStageBytes);
+          mbar_expect_tx(full0 + stage * 8, kStageBytes);
+          tma_load_2d(dst, &tmap, full0 + stage * 8, col, row + part * 64);
+          // the tile's other rows, or the up columns of these
+          tma_load_2d(dst + kBoxBytes, &tmap, full0 + stage * 8, SWIGLU ? K + col : col, SWIGLU ? row + part * 64 : row + 64);
+          advance();
+        }
+      }
+    }
+    return;
+  }
+  const int lane16 = threadIdx.x & 15;
+  const int row_in_pass = threadIdx.x >> 4;
+  int turn = 0;
+  bool ok = true;
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int col = (t % col_tiles) * kMxTileCols + lane16 * 8;
+    const int first = (t / col_tiles) * kMxTileRows + row_in_pass;
+    const int rows_left = col < K ? M - first : 0;          // pass p is stored for p * 16 < rows_left
+    uint32_t* dst = q + (int64_t)first * (K / 8) + col / 8;
+    uint32_t* tile = reinterpret_cast<uint32_t*>(smem + kTileBuf + turn * kMxTileBytes);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      // after a timeout every thread still walks its tiles (and meets the barriers), without waiting
+      if (ok) ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout);
+      const uint4* src = reinterpret_cast<const uint4*>(smem + stage * kStageBytes) + row_in_pass * 16 + lane16;
+#pragma unroll
+      for (int pp = 0; pp < PART_PASSES; ++pp) {
+        const int p = part * PART_PASSES + pp;
+        const uint4 v = src[pp * kRowsPerPass * 16];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        float f[8];
+        uint32_t m;
+        if constexpr (SWIGLU) {
+          const uint4 u = src[kBoxBytes / 16 + pp * kRowsPerPass * 16];
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            unpack2(silu_mul2(bf16x2_to_f32x2(w[i]), bf16x2_to_f32x2(uw[i])), f[2 * i], f[2 * i + 1]);
+          m = col < K ? mx_absmax_halves(f) : 0u;           // past the gate columns lie up columns, not zeros
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) unpack2(bf16x2_to_f32x2(w[i]), f[2 * i], f[2 * i + 1]);
+          m = mx_absmax_bits(mx_absmax_bits(mx_absmax_bits(w[0] & 0x7fff7fffu, w[1]), w[2]), w[3]);
+        }
+        const uint32_t byte = mx_block_byte(m);
+        const uint32_t word = mx_gather_word(byte);
+        if (p * kRowsPerPass < rows_left) dst[(int64_t)p * kRowsPerPass * (K / 8)] = mx_quantize8(f, byte);
+        if (lane16 == 0) tile[mx_scale_offset(p * kRowsPerPass + row_in_pass, 0) / 4] = word;
+      }
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + stage * 8);
+      advance();
+    }
+    // The tile's bytes are complete; the other buffer is written next, and this one again only after
+    // one more of these barriers.
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    if (threadIdx.x < kMxTileBytes / 16)
+      reinterpret_cast<uint4*>(scales + (int64_t)t * kMxTileBytes)[threadIdx.x] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+    turn ^= 1;
+  }
 }
 
 // The values of a quantised matrix in bf16 (exact, but where 6 * 2^e passes bf16's range): the same
 // tile per CTA, four bytes of elements in and 16 bytes out per thread and row.
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 dequantize_mxfp4_kernel(const uint32_t* __restrict__ q, const uint8_t* __restrict__ scales, uint4* __restrict__ out,
                         int M, int K, int col_tiles) {
   const int ct = blockIdx.x % col_tiles;
@@ -186,13 +234,38 @@ int tile_grid(const char* what, int64_t M, int64_t K, int* col_tiles, unsigned* 
 int launch_quantize_mxfp4(const void* x, uint8_t* q, uint8_t* scales, int64_t M, int64_t K, bool swiglu,
                           cudaStream_t stream) {
   int ct;
-  unsigned grid;
-  const int st = tile_grid("quantize_mxfp4", M, K, &ct, &grid);
+  unsigned tiles;
+  const int st = tile_grid("quantize_mxfp4", M, K, &ct, &tiles);
   if (st != B2_OK) return st;
+  static PerDeviceSetup per_device;
+  const DeviceSlot* slot = nullptr;
+  const int setup_status = per_device.get("quantize_mxfp4", [](int dev, DeviceSlot& s) -> int {
+    const void* kernels[2] = {(const void*)quantize_mxfp4_kernel<false>, (const void*)quantize_mxfp4_kernel<true>};
+    for (const void* f : kernels) {
+      const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kQuantSmem);
+      if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "quantize_mxfp4: smem attribute: %s", cudaGetErrorString(e));
+    }
+    s.a = kNumSMsB200;
+    cudaDeviceGetAttribute(&s.a, cudaDevAttrMultiProcessorCount, dev);
+    return B2_OK;
+  }, &slot);
+  if (setup_status != B2_OK) return setup_status;
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B2_LAUNCH_FAILED, "quantize_mxfp4: cuTensorMapEncodeTiled is unavailable");
+  CUtensorMap map;
+  const cuuint64_t width = (cuuint64_t)K * (swiglu ? 2 : 1);
+  const cuuint64_t dims[2] = {width, (cuuint64_t)M}, strides[1] = {width * 2};
+  const cuuint32_t box[2] = {kMxTileCols, 64}, estr[2] = {1, 1};
+  const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "quantize_mxfp4: tensor map encode failed (%d)", (int)r);
+  const unsigned cap = (unsigned)slot->a * 2;
+  const unsigned grid = tiles < cap ? tiles : cap;
   if (swiglu)
-    quantize_mxfp4_kernel<true><<<grid, kThreads, 0, stream>>>((const uint4*)x, (uint32_t*)q, scales, (int)M, (int)K, ct);
+    quantize_mxfp4_kernel<true><<<grid, kThreads + 32, kQuantSmem, stream>>>(map, (uint32_t*)q, scales, (int)M, (int)K, ct, (int)tiles);
   else
-    quantize_mxfp4_kernel<false><<<grid, kThreads, 0, stream>>>((const uint4*)x, (uint32_t*)q, scales, (int)M, (int)K, ct);
+    quantize_mxfp4_kernel<false><<<grid, kThreads + 32, kQuantSmem, stream>>>(map, (uint32_t*)q, scales, (int)M, (int)K, ct, (int)tiles);
   return check_launch("quantize_mxfp4");
 }
 

@@ -16,7 +16,7 @@
 namespace b2 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // of the generic kernel
 
 struct RmsArgs {
   const uint4* x;
@@ -41,11 +41,11 @@ __device__ __forceinline__ float int8_scale(float absmax, float& inv, bool& zero
 // Round half even of a value within +-127 (a few units in the last place over): low byte of the sum.
 __device__ __forceinline__ uint32_t int8_bits(float v) { return __float_as_uint(v + 12582912.0f) & 0xffu; }
 
-template <int TPR, int VPT, bool MX>
-__global__ void __launch_bounds__(kThreads)
+template <int THREADS, int TPR, int VPT, bool MX>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS)
 rmsnorm_residual_kernel(const RmsArgs a) {
-  __shared__ float red[2][kThreads / 32];
-  constexpr int RPC = kThreads / TPR;
+  __shared__ float red[2][THREADS / 32];
+  constexpr int RPC = THREADS / TPR;
   const int slot = threadIdx.x / TPR;
   const int lane = threadIdx.x % TPR;
   uint4 wt[VPT];
@@ -69,6 +69,20 @@ rmsnorm_residual_kernel(const RmsArgs a) {
       v[i] = in ? ldg_stream(a.x + row * a.cvec + c) : make_uint4(0, 0, 0, 0);
       r[i] = in && a.residual != nullptr ? ldg_stream(a.residual + row * a.cvec + c) : make_uint4(0, 0, 0, 0);
     }
+    // The row that this slot takes next is asked into L2 now: between the loads of two rows lie two
+    // dependent reductions, and what is in flight meanwhile is all that keeps memory busy (int8,
+    // 4099 x 5120: 43 -> 31 us, 8192 x 16384: 277 -> 154 us).
+    const int64_t next = row + (int64_t)gridDim.x * RPC;
+    if (next < a.M) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = lane + i * TPR;
+        if (c < a.cvec && (lane & 7) == 0) {   // one request per 128-byte line
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.x + next * a.cvec + c));
+          if (a.residual != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.residual + next * a.cvec + c));
+        }
+      }
+    }
     uint64_t ss2[2] = {0ull, 0ull};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -91,7 +105,7 @@ rmsnorm_residual_kernel(const RmsArgs a) {
     unpack2(ss2[0], a0, a1);
     unpack2(ss2[1], b0, b1);
     // consecutive reductions use the two buffers in turn
-    const float ss = slot_allreduce<kThreads, TPR>((a0 + a1) + (b0 + b1), red[turn], slot, SumOp());
+    const float ss = slot_allreduce<THREADS, TPR>((a0 + a1) + (b0 + b1), red[turn], slot, SumOp());
     turn ^= 1;
     const float rstd = rsqrtf(ss * a.inv_c + a.eps);
     const uint64_t rstd2 = pack2(rstd, rstd);
@@ -101,38 +115,29 @@ rmsnorm_residual_kernel(const RmsArgs a) {
     for (int i = 0; i < VPT; ++i) {
       const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
       const uint32_t ww[4] = {wt[i].x, wt[i].y, wt[i].z, wt[i].w};
-      uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j)
         unpack2(mul2(mul2(bf16x2_to_f32x2(w[j]), rstd2), bf16x2_to_f32x2(ww[j])), y[i][2 * j], y[i][2 * j + 1]);
-        m = max(m, max(__float_as_uint(y[i][2 * j]) & 0x7fffffffu, __float_as_uint(y[i][2 * j + 1]) & 0x7fffffffu));
-      }
       if constexpr (MX) {
         const int c = lane + i * TPR;
         // columns outside the row (and rows outside the matrix) are zeros times rstd: not NaN unless
-        // rstd is one, so they are cleared
-        if (!live || c >= a.cvec) m = 0;
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t byte = mx_scale_byte(m >> 23);
-        const float inv = mx_inverse_scale(byte);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[i][j] *= inv;
-        const uint32_t word = mx_gather_word(byte, 0xffffffffu);
-        if (live && c < a.cvec)
-          reinterpret_cast<uint32_t*>(a.q)[row * a.cvec + c] = byte == 255u ? 0u : mx_pack8(y[i]);
+        // rstd is one, so they are left out
+        const uint32_t byte = mx_block_byte(live && c < a.cvec ? mx_absmax_halves(y[i]) : 0u);
+        const uint32_t word = mx_gather_word(byte);
+        if (live && c < a.cvec) reinterpret_cast<uint32_t*>(a.q)[row * a.cvec + c] = mx_quantize8(y[i], byte);
         if ((c & 15) == 0 && c < col_tiles * 16)
           *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.scale) +
                                        ((row / kMxTileRows) * col_tiles + c / 16) * kMxTileBytes +
                                        mx_scale_offset((int)(row % kMxTileRows), 0)) = word;
       } else {
-        most = max(most, m);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(y[i][j]) & 0x7fffffffu);
       }
     }
     if constexpr (!MX) {
       // the weight's vector of a column outside the row is zero: such columns add nothing to the
       // maximum, but for a NaN that the row's own columns have as well
-      const float absmax = slot_allreduce<kThreads, TPR>(__uint_as_float(most), red[turn], slot, NanMaxOp());
+      const float absmax = slot_allreduce<THREADS, TPR>(__uint_as_float(most), red[turn], slot, NanMaxOp());
       turn ^= 1;
       float inv;
       bool zero_row;
@@ -221,25 +226,28 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
   a.inv_c = inv_c;
   a.eps = eps;
   const int64_t rows = mx ? (M + kMxTileRows - 1) / kMxTileRows * kMxTileRows : M;
-#define B2_RMS(TPR, VPT)                                                                     \
+#define B2_RMS(THREADS, TPR, VPT)                                                            \
   do {                                                                                       \
-    const int64_t need = (rows + kThreads / TPR - 1) / (kThreads / TPR);                     \
-    const int64_t cap = (int64_t)kNumSMsB200 * 8;                                            \
+    const int64_t need = (rows + THREADS / TPR - 1) / (THREADS / TPR);                       \
+    const int64_t cap = (int64_t)kNumSMsB200 * 2048 / THREADS;                               \
     const unsigned g = (unsigned)(need < cap ? need : cap);                                  \
     if (mx)                                                                                  \
-      rmsnorm_residual_kernel<TPR, VPT, true><<<g, kThreads, 0, stream>>>(a);                \
+      rmsnorm_residual_kernel<THREADS, TPR, VPT, true><<<g, THREADS, 0, stream>>>(a);        \
     else                                                                                     \
-      rmsnorm_residual_kernel<TPR, VPT, false><<<g, kThreads, 0, stream>>>(a);               \
+      rmsnorm_residual_kernel<THREADS, TPR, VPT, false><<<g, THREADS, 0, stream>>>(a);       \
   } while (0)
-  // the fewest threads that hold a row at four vectors each (three where that fits exactly)
-  if (C <= 256) B2_RMS(32, 1);
-  else if (C <= 1024) B2_RMS(32, 4);
-  else if (C <= 2048) B2_RMS(64, 4);
-  else if (C <= 3072) B2_RMS(128, 3);
-  else if (C <= 4096) B2_RMS(128, 4);
-  else if (C <= 6144) B2_RMS(256, 3);
-  else if (C <= 8192) B2_RMS(256, 4);
-  else B2_RMS(256, 8);
+  // Two vectors per thread up to 4096 columns (against four: int8 at 23638 x 1024 36 -> 35 us, MXFP4
+  // at 50000 x 2048 131 -> 115 us), where they do not fill a row's threads badly; above, as few
+  // threads as keep a row in registers (8192 columns: 256 threads x 4 82 us, 512 x 2 107 us).
+  if (C <= 256) B2_RMS(256, 32, 1);
+  else if (C <= 512) B2_RMS(256, 32, 2);
+  else if (C <= 1024) B2_RMS(256, 64, 2);
+  else if (C <= 2048) B2_RMS(256, 128, 2);
+  else if (C <= 3072) B2_RMS(256, 128, 3);
+  else if (C <= 4096) B2_RMS(256, 256, 2);
+  else if (C <= 6144) B2_RMS(256, 256, 3);
+  else if (C <= 8192) B2_RMS(256, 256, 4);
+  else B2_RMS(512, 512, 4);
 #undef B2_RMS
   return check_launch("rmsnorm_residual");
 }

@@ -218,3 +218,18 @@ def test_offsets_past_32_bits(cuda_pkg):
     assert torch.equal(q[first:], q2) and torch.equal(s[first // 128:], s2)
     back = ops.dequantize_mxfp4(q, s)
     assert torch.equal(back[first:], ops.dequantize_mxfp4(q2, s2)) and not back[:first].any()
+
+
+def test_swiglu_columns_behind_the_gates_are_not_read_as_gates(cuda_pkg):
+    """K not a multiple of 128: the columns behind the last gate are up columns; infinities there
+    stay in their own blocks and the scale bytes outside the matrix are 0."""
+    m, k = 140, 160
+    x = acts(m, 2 * k, 3).clamp(-20, 20)
+    want_q, want_s = (t.cpu() for t in cuda_pkg.ops.swiglu_quantize_mxfp4(x.to(DEV)))
+    x[5, k + 3] = float("inf")
+    q, s = (t.cpu() for t in cuda_pkg.ops.swiglu_quantize_mxfp4(x.to(DEV)))
+    byte, want = R.mx_bytes(s, m, k), R.mx_bytes(want_s, m, k)
+    assert byte[5, 0] == 255
+    byte[5, 0] = want[5, 0]
+    assert torch.equal(byte, want) and torch.equal(R.mx_tiles(byte), want_s)
+    assert torch.equal(q[:, 16:], want_q[:, 16:]) and not q[5, :16].any()
