@@ -30,6 +30,7 @@
 // Bound by the tensor cores (4 * 128 FLOP per visible pair and head) when many rows share the keys,
 // by reading K and V once for single tokens.
 #include "flash_common.cuh"
+#include "sm100_pair.cuh"
 
 namespace b2 {
 
@@ -42,19 +43,46 @@ using namespace flash;
 constexpr int WIN_REGS_SERVICE = 40;
 static_assert(2 * B2_FLASH_REGS_SOFTMAX + WIN_REGS_SERVICE <= 3 * kLaunchRegs,
               "register split exceeds the CTA's launch allocation");
-constexpr int KV_STAGES = 2;
-constexpr int SMEM_Q = 0;
-constexpr int SMEM_K = SMEM_Q + 2 * TILE_BYTES;
-constexpr int SMEM_V = SMEM_K + KV_STAGES * TILE_BYTES;
-constexpr int SMEM_BARS = SMEM_V + KV_STAGES * TILE_BYTES;
-constexpr int WV_CLEAN = NUM_BARS;                    // [stage]: a mixed tile's values are cleared
-constexpr int WIN_BARS = NUM_BARS + KV_STAGES;
-constexpr int SMEM_TOTAL = 1024 + SMEM_BARS + WIN_BARS * 8 + 16;
+// Shared memory: Q, the K ring, the V ring, barriers.  The few-row form has one tile of Q and a third
+// stage in its place.
+template <bool FEW>
+struct WinSmem {
+  static constexpr int STAGES = FEW ? 3 : 2;
+  static constexpr int Q = 0;
+  static constexpr int K = Q + (FEW ? 1 : 2) * TILE_BYTES;
+  static constexpr int V = K + STAGES * TILE_BYTES;
+  static constexpr int BARS = V + STAGES * TILE_BYTES;
+  // barriers; [stage] or [tile], P by part and tile
+  static constexpr int QF = 0, SF = 2, OF = 4, PF = 6;           // Q, S, O, P are there
+  static constexpr int KF = PF + 2 * P_PARTS, KE = KF + STAGES;  // K is there / has been used
+  static constexpr int VF = KE + STAGES, VE = VF + STAGES;
+  static constexpr int VC = VE + STAGES;                         // a mixed tile's values are cleared
+  static constexpr int NUM = VC + STAGES;
+  static constexpr int TOTAL = 1024 + BARS + NUM * 8 + 16;
+  static_assert(TOTAL <= 227 * 1024, "shared memory budget");
+  // joining the parts of a cluster: each CTA's rows in the place of Q, K and V
+  static constexpr int PITCH = HEAD_DIM + 4;                     // floats: rows start 4 banks apart
+  static constexpr int ML = 2 * BLOCK_M * PITCH * 4;
+  static_assert(ML + 2 * BLOCK_M * 8 <= BARS, "the rows to join take the place of the operands");
+};
 constexpr int kFixWarp = 10, kFixThreads = 64;
+constexpr int kMaxCluster = 8;                // CTAs that join their parts through shared memory
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 
 struct WinArgs {
   __nv_bfloat16* out;           // [B, Sq, H, 128]
-  float* part_o;                // [parts][B * Sq * H][128], null: no parts
+  int join;                     // the cluster's CTAs join their parts
+  float* part_o;                // [parts][B * Sq * H][128]: parts for window_join_kernel, or null
   float2* part_ml;              // [parts][B * Sq * H]: (maximum in the exp2 domain, sum)
   const __nv_bfloat16* q;
   const __nv_bfloat16* v;       // for the non-finite path
@@ -193,16 +221,42 @@ __device__ __forceinline__ bool clean_values(uint32_t tile, int valid, int ft) {
   return found;
 }
 
+// What the sum of a row's parts says about the row: its multiplier, 0 for a row that sees nothing, NaN
+// where the formula has 0 / 0 (keys in sight whose scores are all -inf) or a NaN.
+__device__ __forceinline__ float row_inverse(const WinArgs& a, float l, int p, int n) {
+  if (l == 0.f) return sees_any(a, p, n) ? __uint_as_float(0x7fc00000u) : 0.0f;
+  return 1.0f / l;
+}
+// Joins parts one by one: weights 2^(m - max m).  The first pass finds the maximum.
+struct PartSum {
+  float top = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(const float2& ml, const float4& x) {
+    if (ml.x == -INFINITY && ml.y == 0.f) return;   // this part saw nothing
+    const float w = exp2f(ml.x - top);
+    l = fmaf(w, ml.y, l);
+    o.x = fmaf(w, x.x, o.x);
+    o.y = fmaf(w, x.y, o.y);
+    o.z = fmaf(w, x.z, o.z);
+    o.w = fmaf(w, x.w, o.w);
+  }
+  __device__ __forceinline__ uint2 row(float inv) const {
+    return make_uint2(pack_bf16x2_rn(o.x * inv, o.y * inv), pack_bf16x2_rn(o.z * inv, o.w * inv));
+  }
+};
+
 // FEW: at most 128 rows per key head; the two tiles are two streams over the same rows.
 template <bool FEW>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                   const __grid_constant__ WinArgs args) {
+  using L = WinSmem<FEW>;
+  constexpr int STAGES = L::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SMEM_BARS);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WIN_BARS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::NUM);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* nonfinite = abort_flag + 1;
   const uint32_t sbase = smem_u32(smem);
@@ -218,12 +272,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const int row0 = block * CTA_ROWS;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < WIN_BARS; ++i) {
+    for (int i = 0; i < L::NUM; ++i) {
       int count = 1;
-      if (i == Q_FULL || i == Q_FULL + 1) count = 4;                     // the tile's four warps
-      if (i >= P_PART && i < P_PART + 2 * P_PARTS) count = 4;
-      if (i == V_EMPTY || i == V_EMPTY + 1) count = 1 + kFixThreads / 32;   // MMAs done, looked through
-      if (i >= WV_CLEAN) count = kFixThreads;
+      if (i < L::SF || (i >= L::PF && i < L::KF)) count = 4;             // the tile's four warps
+      if (i >= L::VE && i < L::VC) count = 1 + kFixThreads / 32;         // MMAs done, looked through
+      if (i >= L::VC) count = kFixThreads;
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -247,14 +300,27 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WIN_REGS_SERVICE));
     if (warp == kLoadWarp) {
       if (lane == 0) {
-        for (int j = 0; j < steps; ++j) {
-          const int st = j & 1;
-          const uint32_t par = ((j >> 1) & 1) ^ 1;
-          const int key0 = step_key(span, j);
-          if (!mbar_wait(bar(K_EMPTY + st), par, abort_flag, kStatusFlashTimeout)) break;
-          load_tile(sbase + SMEM_K + st * TILE_BYTES, &tmap_k, bar(K_FULL + st), key0, hkv, b, args.k_swap);
-          if (!mbar_wait(bar(V_EMPTY + st), par, abort_flag, kStatusFlashTimeout)) break;
-          load_tile(sbase + SMEM_V + st * TILE_BYTES, &tmap_v, bar(V_FULL + st), key0, hkv, b, args.v_swap);
+        auto load_k = [&](int j) -> bool {
+          const int st = j % STAGES;
+          if (!mbar_wait(bar(L::KE + st), ((j / STAGES) & 1) ^ 1, abort_flag, kStatusFlashTimeout)) return false;
+          load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), step_key(span, j), hkv, b, args.k_swap);
+          return true;
+        };
+        auto load_v = [&](int j) -> bool {
+          const int st = j % STAGES;
+          if (!mbar_wait(bar(L::VE + st), ((j / STAGES) & 1) ^ 1, abort_flag, kStatusFlashTimeout)) return false;
+          load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), step_key(span, j), hkv, b, args.v_swap);
+          return true;
+        };
+        // In the few-row form a step's K is free long before its V (the streams' MMAs alternate), so
+        // K runs a step ahead: behind V it would wait for the other stream's product as well.
+        bool ok = steps == 0 || !FEW || load_k(0);
+        for (int j = 0; ok && j < steps; ++j) {
+          if constexpr (FEW)
+            ok = j + 1 >= steps || load_k(j + 1);
+          else
+            ok = load_k(j);
+          ok = ok && load_v(j);
         }
       }
     } else if (warp >= kFixWarp) {
@@ -263,35 +329,40 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       // the ring by a whole phase nor fall behind it by one
       for (int j = 0; j < steps; ++j) {
         const int key0 = step_key(span, j);
-        const int st = j & 1;
-        if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1, abort_flag, kStatusFlashTimeout)) break;
+        const int st = j % STAGES;
+        if (!mbar_wait(bar(L::VF + st), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) break;
         if (is_mixed(args, span, key0)) {
-          if (clean_values(sbase + SMEM_V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
+          if (clean_values(sbase + L::V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
           fence_proxy_async_smem();
-          mbar_arrive(bar(WV_CLEAN + st));
+          mbar_arrive(bar(L::VC + st));
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(V_EMPTY + st));
+        if (lane == 0) mbar_arrive(bar(L::VE + st));
       }
     } else if (warp == kMmaWarp && steps > 0) {
       const bool leader = elect_one() != 0;
       const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // tile 1: 128 columns on
-      const uint32_t q0 = desc_lo(sbase + SMEM_Q, 16);
-      const uint32_t k0 = desc_lo(sbase + SMEM_K, 16);
-      const uint32_t v0 = desc_lo(sbase + SMEM_V, HALF_BYTES);
+      const uint32_t q0 = desc_lo(sbase + L::Q, 16);
+      const uint32_t k0 = desc_lo(sbase + L::K, 16);
+      const uint32_t v0 = desc_lo(sbase + L::V, HALF_BYTES);
       constexpr uint32_t TILE_UNITS = TILE_BYTES >> 4;
       uint32_t clean_phase = 0;   // bit per stage
       // S of tile t = Q . K^T of the stage's keys
       auto issue_qk = [&](int t, int st) {
         if (leader) mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + (FEW ? 0 : t) * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
-        if (leader) tc_commit(bar(S_FULL + t));
+        if (leader) tc_commit(bar(L::SF + t));
       };
-      // the stage's values are there, and cleared if the tile is mixed
+      auto wait_k = [&](int j) -> bool {
+        if (!mbar_wait(bar(L::KF + j % STAGES), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) return false;
+        tc_fence_after();
+        return true;
+      };
+      // the step's values are there, and cleared if the tile is mixed
       auto wait_v = [&](int j) -> bool {
-        const int st = j & 1;
-        if (!mbar_wait(bar(V_FULL + st), (j >> 1) & 1, abort_flag, kStatusFlashTimeout)) return false;
+        const int st = j % STAGES;
+        if (!mbar_wait(bar(L::VF + st), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) return false;
         if (is_mixed(args, span, step_key(span, j))) {
-          if (!mbar_wait(bar(WV_CLEAN + st), (clean_phase >> st) & 1, abort_flag, kStatusFlashTimeout)) return false;
+          if (!mbar_wait(bar(L::VC + st), (clean_phase >> st) & 1, abort_flag, kStatusFlashTimeout)) return false;
           clean_phase ^= 1u << st;
         }
         return true;
@@ -300,7 +371,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       auto issue_pv = [&](int t, int st, int use) -> bool {
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          if (!mbar_wait(bar(P_PART + 2 * part + t), use & 1, abort_flag, kStatusFlashTimeout)) return false;
+          if (!mbar_wait(bar(L::PF + 2 * part + t), use & 1, abort_flag, kStatusFlashTimeout)) return false;
           tc_fence_after();
           if (leader) {
             if (part == 0)
@@ -312,45 +383,38 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         return true;
       };
       static_assert(P_PARTS == 2, "P is published in halves");
-      bool ok = mbar_wait(bar(Q_FULL), 0, abort_flag, kStatusFlashTimeout) &&
-                mbar_wait(bar(K_FULL), 0, abort_flag, kStatusFlashTimeout);
+      bool ok = mbar_wait(bar(L::QF), 0, abort_flag, kStatusFlashTimeout) && wait_k(0);
       if constexpr (FEW) {
-        // step j belongs to stream j & 1, which is also its ring stage
+        // step j belongs to stream j & 1
         if (ok) {
-          tc_fence_after();
           issue_qk(0, 0);
-          if (leader) tc_commit(bar(K_EMPTY));
+          if (leader) tc_commit(bar(L::KE));
         }
-        if (ok && steps > 1) {
-          ok = mbar_wait(bar(K_FULL + 1), 0, abort_flag, kStatusFlashTimeout);
-          if (ok) {
-            issue_qk(1, 1);
-            if (leader) tc_commit(bar(K_EMPTY + 1));
-          }
+        if (ok && steps > 1 && (ok = wait_k(1))) {
+          issue_qk(1, 1);
+          if (leader) tc_commit(bar(L::KE + 1));
         }
         for (int j = 0; ok && j < steps; ++j) {
           const int t = j & 1;
-          if (!(ok = wait_v(j) && issue_pv(t, t, j >> 1))) break;
-          if (leader) tc_commit(bar(V_EMPTY + t));
+          if (!(ok = wait_v(j) && issue_pv(t, j % STAGES, j >> 1))) break;
+          if (leader) tc_commit(bar(L::VE + j % STAGES));
           if (j + 2 < steps) {
-            if (!(ok = mbar_wait(bar(K_FULL + t), ((j + 2) >> 1) & 1, abort_flag, kStatusFlashTimeout))) break;
-            tc_fence_after();
-            issue_qk(t, t);
-            if (leader) tc_commit(bar(K_EMPTY + t));
+            if (!(ok = wait_k(j + 2))) break;
+            issue_qk(t, (j + 2) % STAGES);
+            if (leader) tc_commit(bar(L::KE + (j + 2) % STAGES));
           } else {
-            if (leader) tc_commit(bar(O_FULL + t));
+            if (leader) tc_commit(bar(L::OF + t));
           }
         }
       } else {
         if (ok) {
-          tc_fence_after();
           issue_qk(0, 0);
-          ok = mbar_wait(bar(Q_FULL + 1), 0, abort_flag, kStatusFlashTimeout);
+          ok = mbar_wait(bar(L::QF + 1), 0, abort_flag, kStatusFlashTimeout);
         }
         if (ok) {
           tc_fence_after();
           issue_qk(1, 0);
-          if (leader) tc_commit(bar(K_EMPTY));
+          if (leader) tc_commit(bar(L::KE));
           ok = wait_v(0);
         }
         for (int j = 0; ok && j < steps; ++j) {
@@ -358,24 +422,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           const bool last = j + 1 == steps;
           if (!(ok = issue_pv(0, st, j))) break;
           if (last) {
-            if (leader) tc_commit(bar(O_FULL));
+            if (leader) tc_commit(bar(L::OF));
           } else {
-            if (!(ok = mbar_wait(bar(K_FULL + (st ^ 1)), ((j + 1) >> 1) & 1, abort_flag, kStatusFlashTimeout))) break;
-            tc_fence_after();
+            if (!(ok = wait_k(j + 1))) break;
             issue_qk(0, st ^ 1);
           }
           if (!(ok = issue_pv(1, st, j))) break;
-          if (leader) tc_commit(bar(V_EMPTY + st));
+          if (leader) tc_commit(bar(L::VE + st));
           if (last) {
-            if (leader) tc_commit(bar(O_FULL + 1));
+            if (leader) tc_commit(bar(L::OF + 1));
           } else {
             // the next step's values, waited for while this step's MMAs are still queued
             if (!(ok = wait_v(j + 1))) break;
             issue_qk(1, st ^ 1);
-            if (leader) tc_commit(bar(K_EMPTY + (st ^ 1)));
+            if (leader) tc_commit(bar(L::KE + (st ^ 1)));
           }
         }
       }
+    }
+    if (args.join) {   // the softmax warps' two meetings
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(B2_FLASH_REGS_SOFTMAX));
@@ -398,11 +466,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
       for (int p = 0; p < 16; ++p) {
         const int r = p * 8 + (tid >> 4);
-        sts128(sbase + SMEM_Q + t * TILE_BYTES + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
+        sts128(sbase + L::Q + t * TILE_BYTES + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(Q_FULL + t));
+      if (lane == 0) mbar_arrive(bar(L::QF + t));
     }
     const int uses = FEW ? (steps + 1 - t) >> 1 : steps;   // steps of this tile (stream)
     const int row = tile_row0 + quarter * 32 + lane;
@@ -421,14 +489,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     bool ok = true;
     float row_max = -INFINITY, row_sum = 0.f;
     for (int u = 0; u < uses; ++u) {
-      if (ok) ok = mbar_wait(bar(S_FULL + t), u & 1, abort_flag, kStatusFlashTimeout);
+      if (ok) ok = mbar_wait(bar(L::SF + t), u & 1, abort_flag, kStatusFlashTimeout);
       tc_fence_after();
       if (!warp_ok) {   // none of the warp's rows exist: whatever P holds there goes nowhere
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(bar(P_PART + t));
-          mbar_arrive(bar(P_PART + 2 + t));
+          mbar_arrive(bar(L::PF + t));
+          mbar_arrive(bar(L::PF + 2 + t));
         }
         continue;
       }
@@ -482,7 +550,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(P_PART + 2 * (q / 4) + t));
+          if (lane == 0) mbar_arrive(bar(L::PF + 2 * (q / 4) + t));
         }
       }
       float a0, a1, b0, b1, c0, c1, d0, d1;
@@ -492,20 +560,26 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       unpack2(sm2[3], d0, d1);
       row_sum += ((a0 + a1) + (b0 + b1)) + ((c0 + c1) + (d0 + d1));
     }
-    if (ok && uses > 0) ok = mbar_wait(bar(O_FULL + t), 0, abort_flag, kStatusFlashTimeout);
+    if (ok && uses > 0) ok = mbar_wait(bar(L::OF + t), 0, abort_flag, kStatusFlashTimeout);
+    // the rows to join take the operands' place: no MMA of the other tile may still read them
+    const int other_uses = FEW ? (steps + t) >> 1 : steps;
+    if (ok && args.join && other_uses > 0) ok = mbar_wait(bar(L::OF + (t ^ 1)), 0, abort_flag, kStatusFlashTimeout);
     // without parts the few-row form has a single step, which is stream 0's
-    if (ok && warp_ok && !(FEW && t == 1 && args.part_o == nullptr)) {
+    const bool parts = args.part_o != nullptr;
+    if (ok && warp_ok && !(FEW && t == 1 && !parts && !args.join)) {
       tc_fence_after();
       const int h = hkv * args.share + (my_row - my_i * args.share);
       const int64_t out_row = ((int64_t)b * args.Sq + my_i) * args.H + h;
-      const bool parts = args.part_o != nullptr;
       const int part = FEW ? 2 * split + t : split;
-      // keys in sight whose scores are all -inf leave 0 / 0, as the formula does
-      const float inv = parts ? 1.0f
-                        : row_sum == 0.f ? (sees_any(args, p_row, span.n) ? __uint_as_float(0x7fc00000u) : 0.0f)
-                        : row_sum != row_sum ? 1.0f : 1.0f / row_sum;
-      if (parts && row_ok)
-        args.part_ml[part * args.total_rows + out_row] = make_float2(row_max * sl2, row_sum);
+      const float inv = parts || args.join || row_sum != row_sum ? 1.0f : row_inverse(args, row_sum, p_row, span.n);
+      const int slot = t * BLOCK_M + quarter * 32 + lane;
+      if (row_ok) {
+        const float2 ml = make_float2(row_max * sl2, row_sum);
+        if (args.join)
+          reinterpret_cast<float2*>(smem + L::ML)[slot] = ml;
+        else if (parts)
+          args.part_ml[part * args.total_rows + out_row] = ml;
+      }
       const bool fix = *nonfinite != 0;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
@@ -533,10 +607,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           }
         }
         if (!row_ok) continue;
-        if (parts) {
-          uint4* dst = reinterpret_cast<uint4*>(args.part_o + (part * args.total_rows + out_row) * HEAD_DIM + c);
+        if (parts || args.join) {
+          float* dst = args.join ? reinterpret_cast<float*>(smem) + slot * L::PITCH + c
+                                 : args.part_o + (part * args.total_rows + out_row) * HEAD_DIM + c;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         } else {
           uint4* dst = reinterpret_cast<uint4*>(args.out + out_row * HEAD_DIM + c);
 #pragma unroll
@@ -550,6 +626,33 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           }
         }
       }
+    }
+    if (args.join) {
+      __syncwarp();
+      cluster_sync_all();   // every CTA's rows are in its shared memory
+      // a warp takes a row, a lane four columns; the rows go round the cluster's CTAs
+      const int nrows = min(CTA_ROWS, args.rows - row0);
+      for (int r = warp * args.splits + split; r < nrows; r += kSoftmaxWarps * args.splits) {
+        PartSum sum;
+        bool any_nan = false;
+        for (int p = 0; p < (FEW ? 2 : 1) * args.splits; ++p) {
+          const int slot = FEW ? (p & 1) * BLOCK_M + r : r;
+          const float2 ml = ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, FEW ? p >> 1 : p));
+          sum.top = fmaxf(sum.top, ml.x);
+          any_nan |= ml.y != ml.y;
+        }
+        for (int p = 0; p < (FEW ? 2 : 1) * args.splits; ++p) {
+          const int slot = FEW ? (p & 1) * BLOCK_M + r : r;
+          const int cta = FEW ? p >> 1 : p;
+          sum.add(ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, cta)),
+                  ld_cluster_f4(map_to_cta(sbase + (slot * L::PITCH + lane * 4) * 4, cta)));
+        }
+        const int i = (row0 + r) / args.share, h = hkv * args.share + (row0 + r) % args.share;
+        const float inv = any_nan ? __uint_as_float(0x7fc00000u) : row_inverse(args, sum.l, i + span.n - args.Sq, span.n);
+        reinterpret_cast<uint2*>(args.out + (((int64_t)b * args.Sq + i) * args.H + h) * HEAD_DIM)[lane] = sum.row(inv);
+      }
+      __syncwarp();
+      cluster_sync_all();   // no CTA retires while another reads its rows
     }
   }
 
@@ -567,48 +670,36 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
 }
 
-// Joins the parts of each row: weights 2^(m - max m), one warp per row, four columns per lane.
+// Joins the parts that lie in memory: one warp per row, four columns per lane.
 __global__ void __launch_bounds__(256)
 window_join_kernel(const WinArgs args, int parts) {
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= args.total_rows) return;
-  float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, args.part_ml[p * args.total_rows + row].x);
-  float l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  PartSum sum;
   bool any_nan = false;
-  for (int p = 0; p < parts; ++p) {
+  for (int p = lane; p < parts; p += 32) {
     const float2 ml = args.part_ml[p * args.total_rows + row];
+    sum.top = fmaxf(sum.top, ml.x);
     any_nan |= ml.y != ml.y;
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;   // this part saw nothing
-    const float w = exp2f(ml.x - top);
-    const float4 x = reinterpret_cast<const float4*>(args.part_o + (p * args.total_rows + row) * HEAD_DIM)[lane];
-    l = fmaf(w, ml.y, l);
-    o.x = fmaf(w, x.x, o.x);
-    o.y = fmaf(w, x.y, o.y);
-    o.z = fmaf(w, x.z, o.z);
-    o.w = fmaf(w, x.w, o.w);
   }
-  float inv = 1.0f / l;
-  if (any_nan) {
-    inv = __uint_as_float(0x7fc00000u);
-  } else if (l == 0.f) {
-    const int64_t bi = row / args.H;
-    const int b = (int)(bi / args.Sq), i = (int)(bi - (int64_t)b * args.Sq);
-    const int n = sequence_keys(args.lengths, b, args.Sk);
-    inv = sees_any(args, i + n - args.Sq, n) ? __uint_as_float(0x7fc00000u) : 0.f;
-  }
-  uint2 w;
-  w.x = pack_bf16x2_rn(o.x * inv, o.y * inv);
-  w.y = pack_bf16x2_rn(o.z * inv, o.w * inv);
-  reinterpret_cast<uint2*>(args.out + row * HEAD_DIM)[lane] = w;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum.top = fmaxf(sum.top, __shfl_xor_sync(0xffffffffu, sum.top, off));
+  any_nan = __any_sync(0xffffffffu, any_nan);
+  for (int p = 0; p < parts; ++p)
+    sum.add(args.part_ml[p * args.total_rows + row],
+            reinterpret_cast<const float4*>(args.part_o + (p * args.total_rows + row) * HEAD_DIM)[lane]);
+  const int64_t bi = row / args.H;
+  const int b = (int)(bi / args.Sq), i = (int)(bi - (int64_t)b * args.Sq);
+  const int n = sequence_keys(args.lengths, b, args.Sk);
+  const float inv = any_nan ? __uint_as_float(0x7fc00000u) : row_inverse(args, sum.l, i + n - args.Sq, n);
+  reinterpret_cast<uint2*>(args.out + row * HEAD_DIM)[lane] = sum.row(inv);
 }
 
 // How a call is laid over the GPU: few-row form or not, splits of the key sequence, parts to join.
 struct WinPlan {
-  bool few;
-  int blocks, splits, parts;
+  bool few, join;
+  int blocks, splits, parts;   // parts: to be joined by window_join_kernel (1: none)
 };
 WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks) {
   WinPlan p;
@@ -625,22 +716,39 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
   int64_t steps = (keys + BLOCK_N - 1) / BLOCK_N + (keys < Sk ? 1 : 0);
   if (left >= 0) steps += (min(sinks, Sk) + BLOCK_N - 1) / BLOCK_N;
   steps = max((int64_t)1, min(steps, ((int64_t)Sk + BLOCK_N - 1) / BLOCK_N));
-  // One CTA runs per SM, so a grid takes ceil(CTAs / SMs) rounds of (steps / splits + a fixed part
-  // worth about three steps: set-up, first loads, output).  Splitting pays while it fills empty SMs.
+  // One CTA runs per SM, so a grid takes rounds of (its steps + a fixed part: set-up, first loads,
+  // output).  The figures are microseconds measured on a B200 with 24, 48 and 96 CTAs before
+  // splitting: a few-row step takes 0.83 alone and what 64 KB per CTA take from memory when many run; a
+  // full step 1.85.  A cluster joins its parts for one (few rows) or seven (256 rows), but leaves
+  // SMs without a place; parts in memory take a second kernel and 1040 bytes per row and part, there
+  // and back.  For 24 heads' single tokens over 8192 keys: 65.6 us unsplit, 32.8 in clusters of four,
+  // 35.8 in four parts through memory.
+  constexpr int kSlots[kMaxCluster + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
   const int64_t ctas = (int64_t)p.blocks * Hkv * B;
-  int64_t best = INT64_MAX;
+  double best = 1e30;
   p.splits = 1;
-  for (int s = 1; s <= 64 && s <= steps; ++s) {
-    const int64_t rounds = (ctas * s + kNumSMsB200 - 1) / kNumSMsB200;
-    // parts cost: writing and joining them, about two steps' time per call
-    const int64_t cost = rounds * ((steps + s - 1) / s + 3) + (s > 1 ? 2 : 0);
+  p.join = false;
+  auto consider = [&](int s, bool cluster) {
+    const int64_t n = ctas * s, slots = cluster ? kSlots[s] : kNumSMsB200;
+    const double rounds = (double)((n + slots - 1) / slots);
+    const double running = (double)(n < slots ? n : slots);
+    const double step = p.few ? (running * 0.0109 > 0.83 ? running * 0.0109 : 0.83) : 1.85;
+    double cost = rounds * ((double)steps / s * step + (p.few ? 8.0 : 5.0));
+    if (cluster && (s > 1 || p.few)) cost += p.few ? 1.0 : 7.0 * rounds;
+    if (!cluster) cost += 6.0 + 2.1e-4 * (double)(rows * Hkv * B) * s * (p.few ? 2 : 1);
     if (cost < best) {
       best = cost;
       p.splits = s;
+      p.join = cluster;
     }
+  };
+  for (int s = 1; s <= 64 && s <= steps; ++s) {
+    if (s <= kMaxCluster) consider(s, true);
+    if (s > 1) consider(s, false);
   }
-  p.parts = p.splits * (p.few ? 2 : 1);
-  if (p.few && steps == 1) p.parts = 1;   // the second stream has nothing
+  p.parts = p.join ? 1 : p.splits * (p.few ? 2 : 1);
+  // nothing to join: whole rows of one CTA, or a few-row call of one step (its second stream has none)
+  if (p.join && p.splits == 1 && (!p.few || steps == 1)) p.join = false;
   return p;
 }
 
@@ -658,8 +766,10 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   const DeviceSlot* slot = nullptr;
   const int setup_status = per_device.get("window_fwd", [](int, DeviceSlot&) -> int {
     const void* kernels[2] = {(const void*)window_fwd_kernel<false>, (const void*)window_fwd_kernel<true>};
-    for (const void* f : kernels) {
-      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL);
+    const int bytes[2] = {WinSmem<false>::TOTAL, WinSmem<true>::TOTAL};
+    for (int i = 0; i < 2; ++i) {
+      const void* f = kernels[i];
+      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes[i]);
       if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "window_fwd: smem attribute: %s", cudaGetErrorString(e));
       cudaFuncAttributes fa;
       e = cudaFuncGetAttributes(&fa, f);
@@ -680,6 +790,7 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   if (st != B2_OK) return st;
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.total_rows = (int64_t)B * Sq * H;
+  a.join = plan.join ? 1 : 0;
   a.part_o = plan.parts == 1 ? nullptr : reinterpret_cast<float*>(workspace);
   a.part_ml = plan.parts == 1 ? nullptr : reinterpret_cast<float2*>(a.part_o + plan.parts * a.total_rows * HEAD_DIM);
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
@@ -702,13 +813,25 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   a.sinks = left < 0 ? 0 : sinks;
   a.splits = plan.splits;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  const dim3 grid(plan.blocks * plan.splits, Hkv, B);
-  if (plan.few)
-    window_fwd_kernel<true><<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(tk, tv, a);
-  else
-    window_fwd_kernel<false><<<grid, NUM_THREADS, SMEM_TOTAL, stream>>>(tk, tv, a);
-  st = check_launch("window_fwd");
-  if (st != B2_OK || plan.parts == 1) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(plan.blocks * plan.splits), (unsigned)Hkv, (unsigned)B);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = plan.few ? WinSmem<true>::TOTAL : WinSmem<false>::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = plan.join ? (unsigned)plan.splits : 1u;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = plan.few ? cudaLaunchKernelEx(&cfg, window_fwd_kernel<true>, tk, tv, a)
+                                 : cudaLaunchKernelEx(&cfg, window_fwd_kernel<false>, tk, tv, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(B2_LAUNCH_FAILED, "window_fwd: launch failed: %s", cudaGetErrorString(e));
+  }
+  if (plan.parts == 1) return B2_OK;
   window_join_kernel<<<(unsigned)((a.total_rows + 7) / 8), 256, 0, stream>>>(a, plan.parts);
   return check_launch("window_fwd (join)");
 }

@@ -167,6 +167,21 @@ def test_long_cache_offsets_past_32_bits(cuda_pkg):
         assert ((a[:, -3:].double() - want).abs() <= bound(want, q, k[:, -3:, -1300:], v[:, -3:, -1300:])).all()
 
 
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,memory", [(1, 2, 2, 1, 65536, True), (1, 3, 1, 40, 50000, True), (1, 24, 24, 836, 9000, True),
+                                                  (1, 1, 1, 300, 30000, True), (1, 24, 24, 1, 8192, False),
+                                                  (1, 24, 6, 3, 8000, False), (1, 8, 8, 256, 2000, False)])
+def test_every_way_to_join_the_parts(cuda_pkg, B, H, Hkv, Sq, Sk, memory):
+    """Key sequences split over a cluster, or through memory, by few rows and by whole tiles."""
+    need = cuda_pkg.ops._window_workspace(B, H, Hkv, Sq, Sk, -1, 0, 0)
+    assert (need > 0) == memory
+    q, k, v = qkv(B, H, Hkv, Sq, Sk, 17)
+    check(cuda_pkg, q, k, v, -1, 0)
+    check(cuda_pkg, q, k, v, 9000, 0, 3)
+    lengths = torch.full((B,), Sk * 2 // 3, dtype=torch.int32, device=DEV)
+    check(cuda_pkg, q, k, v, -1, 0, 0, lengths)
+    check(cuda_pkg, q, k, v, -1, 5, 0, lengths * 0 + 100)            # most parts have nothing to do
+
+
 def test_side_stream_two_captures_and_lengths_that_change(cuda_pkg):
     """Single tokens captured twice in graphs that are replayed in turn while the lengths grow."""
     ops = cuda_pkg.ops

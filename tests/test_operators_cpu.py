@@ -105,10 +105,10 @@ def test_window_arguments_are_checked_before_launch(pkg):
     assert call(v=ODD) == 3 and call(lengths=ODD) == 3
     assert call(ks=[1 << 20, 100, 512]) == 3 and call(vs=[1 << 20, 0, 512]) == 3 and call(qs=[1 << 20, -128, 512]) == 3
     assert call(ks=[1 << 20, 1 << 38, 512]) == 8 and call(B=65536) == 8 and call(Sq=1 << 29) == 8
-    # single tokens of a long cache need room for their parts
+    # single tokens of a few heads over a very long cache leave their parts in memory
     need = ctypes.c_int64(-1)
-    assert lib.b2_window_fwd_workspace(1, 4, 4, 1, 8192, -1, 0, 0, ctypes.byref(need)) == 0 and need.value > 0
-    assert call(Sq=1, Sk=8192, left=-1, right=0, ws=FAKE, ws_bytes=need.value - 1) == 2
+    assert lib.b2_window_fwd_workspace(1, 2, 2, 1, 65536, -1, 0, 0, ctypes.byref(need)) == 0 and need.value > 0
+    assert call(H=2, Hkv=2, Sq=1, Sk=65536, left=-1, right=0, ws=FAKE, ws_bytes=need.value - 1) == 2
     assert b"workspace" in lib.b2_last_error()
     assert lib.b2_window_fwd_workspace(8, 24, 24, 4096, 4096, -1, 0, 0, ctypes.byref(need)) == 0 and need.value == 0
     assert lib.b2_window_fwd_workspace(1, 4, 4, 1, 8192, -1, 0, 0, None) == 7
