@@ -221,6 +221,11 @@ __device__ __forceinline__ bool clean_values(uint32_t tile, int valid, int ft) {
   return found;
 }
 
+// Bits 0 .. n-1 of a word (all for n >= 32, none for n <= 0).
+__device__ __forceinline__ uint32_t columns_below(int n) {
+  return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32));
+}
+
 // What the sum of a row's parts says about the row: its multiplier, 0 for a row that sees nothing, NaN
 // where the formula has 0 / 0 (keys in sight whose scores are all -inf) or a NaN.
 __device__ __forceinline__ float row_inverse(const WinArgs& a, float l, int p, int n) {
@@ -509,9 +514,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         const int key0 = step_key(span, FEW ? 2 * u + t : u);
         const int last = key_last - key0, first = key_first - key0, sink = args.sinks - key0;
         if (__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N))) {
+          // a bit per visible column, 32 at a time: testing constant bits of a word costs a third of
+          // three comparisons per score
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c > last || (c < first && c >= sink)) s[c] = 0xff800000u;   // -inf
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t seen = columns_below(last + 1 - 32 * w) & (~columns_below(first - 32 * w) | columns_below(sink - 32 * w));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(seen & (1u << i))) s[32 * w + i] = 0xff800000u;   // -inf
+          }
         }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
