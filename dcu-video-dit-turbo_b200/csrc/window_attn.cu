@@ -9,10 +9,8 @@
 // exponentials on the FMA pipe, rescaling only when the running maximum grows by more than 2^8);
 // flash_common.cuh holds the shared pieces.  What differs:
 //
-//   rows      The H / Hkv query heads that share a key head are packed with the positions, row
-//             r = i * (H / Hkv) + head, so a CTA's rows read one set of keys and span few positions.
-//             Rows are fetched with plain 16-byte loads into the swizzled tile (any strides, any
-//             packing).
+//   rows      Query heads that share a key head are packed with the positions, row r = i * pack + head,
+//             so a CTA's rows read one set of keys and span few positions.
 //   keys      A CTA walks only the 128-key tiles that some row of it sees: the tiles of the first
 //             keys, then those of its window.  Scores are masked in the tiles that some row does
 //             not see whole ("mixed"); the others take flash_fwd.cu's path.
@@ -21,11 +19,16 @@
 //             at or past n (a cache's unwritten part) and set non-finite values to zero.  Those of
 //             visible keys are added back to the rows that see them at the end (a path that only
 //             runs if there were any).
-//   few rows  With at most 128 rows per key head (single tokens) the two query tiles become two
-//             streams over the same rows: stream 0 takes the even tiles, stream 1 the odd ones, and
-//             the key sequence is split over CTAs as well.  Each stream leaves its maximum, sum and
-//             unnormalised output; a second kernel joins them.  Larger calls whose grid would leave
-//             SMs empty are split the same way.
+//   tiles     window_tile_kernel: two tiles of up to 128 rows per work item.  A CTA that has finished
+//             its item takes over one that has not started (cluster launch control), so loads, first
+//             scores and set-up of the next item run under the output of the last: windows are a
+//             dozen steps long, and starting a CTA costs three.
+//   few rows  window_few_kernel, at most 128 rows per key head (single tokens): the two tiles become
+//             two streams over the same rows, stream 0 takes the even tiles of keys and stream 1 the
+//             odd ones.
+//   splits    Where that leaves SMs empty the keys are split over CTAs.  Parts (maximum, sum, unnormalised
+//             output of each row) are joined in the shared memory of a cluster, or, when there are
+//             many, through memory by a second kernel.
 //
 // Bound by the tensor cores (4 * 128 FLOP per visible pair and head) when many rows share the keys,
 // by reading K and V once for single tokens.
@@ -40,8 +43,12 @@ namespace {
 
 using namespace flash;
 
-constexpr int WIN_REGS_SERVICE = 40;
-static_assert(2 * B2_FLASH_REGS_SOFTMAX + WIN_REGS_SERVICE <= 3 * kLaunchRegs,
+// Registers per thread of the softmax and the service warps (setmaxnreg; see flash_common.cuh for what
+// bounds them).  The work loop of window_tile_kernel's service warps spills below 56 (216 / 72 takes 3 %
+// less time than 232 / 40 over a clip of 23638 tokens).
+constexpr int TILE_REGS_SOFTMAX = 216, TILE_REGS_SERVICE = 72;
+constexpr int FEW_REGS_SOFTMAX = 232, FEW_REGS_SERVICE = 40;
+static_assert(2 * TILE_REGS_SOFTMAX + TILE_REGS_SERVICE <= 3 * kLaunchRegs && 2 * FEW_REGS_SOFTMAX + FEW_REGS_SERVICE <= 3 * kLaunchRegs,
               "register split exceeds the CTA's launch allocation");
 // Shared memory: Q, the K ring, the V ring, barriers.  The few-row form has one tile of Q and a third
 // stage in its place.
@@ -51,19 +58,24 @@ struct WinSmem {
   static constexpr int Q = 0;
   static constexpr int K = Q + (FEW ? 1 : 2) * TILE_BYTES;
   static constexpr int V = K + STAGES * TILE_BYTES;
-  static constexpr int BARS = V + STAGES * TILE_BYTES;
+  static constexpr int NEXT = V + STAGES * TILE_BYTES;           // answers of the work scheduler (2 x 16)
+  static constexpr int BARS = NEXT + 32;
   // barriers; [stage] or [tile], P by part and tile
-  static constexpr int QF = 0, SF = 2, OF = 4, PF = 6;           // Q, S, O, P are there
+  static constexpr int QF = 0, SF = 2, OF = 4;                   // Q, S, O are there
+  static constexpr int OE = 6, QE = 8;                           // O has been read / Q has been used
+  static constexpr int NF = 9, NE = 11;                          // the next item is known / has been read
+  static constexpr int PF = 13;
   static constexpr int KF = PF + 2 * P_PARTS, KE = KF + STAGES;  // K is there / has been used
   static constexpr int VF = KE + STAGES, VE = VF + STAGES;
   static constexpr int VC = VE + STAGES;                         // a mixed tile's values are cleared
   static constexpr int NUM = VC + STAGES;
   static constexpr int TOTAL = 1024 + BARS + NUM * 8 + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
+  static_assert(OE == OF + 2 && QE == OE + 2 && NF == QE + 1 && NE == NF + 2 && PF == NE + 2, "barriers follow one another");
   // joining the parts of a cluster: each CTA's rows in the place of Q, K and V
   static constexpr int PITCH = HEAD_DIM + 4;                     // floats: rows start 4 banks apart
   static constexpr int ML = 2 * BLOCK_M * PITCH * 4;
-  static_assert(ML + 2 * BLOCK_M * 8 <= BARS, "the rows to join take the place of the operands");
+  static_assert(ML + 2 * BLOCK_M * 8 <= NEXT, "the rows to join take the place of the operands");
 };
 constexpr int kFixWarp = 10, kFixThreads = 64;
 constexpr int kMaxCluster = 8;                // CTAs that join their parts through shared memory
@@ -88,19 +100,37 @@ struct WinArgs {
   const __nv_bfloat16* v;       // for the non-finite path
   const int* lengths;           // keys per sequence, null: Sk
   int64_t q_b, q_h, q_s, v_b, v_h, v_s;   // strides in elements
-  int H, Hkv, share, Sq, Sk, rows;        // share = H / Hkv, rows = Sq * share
+  int H, share, Sq, Sk;                   // share = H / Hkv
+  int pack, tile_pos, blocks;             // heads per row group; positions per tile; work items along positions
   int left, right, sinks, splits;
   int64_t total_rows;                     // B * Sq * H
   int k_swap, v_swap;
   float scale_log2;
 };
 
+// One work item: positions [pos0, pos0 + CTA positions) of `pack` heads from h0, a share of their keys.
+struct Item {
+  int split, block, h0, hkv, b;
+};
+__device__ __forceinline__ Item decode_item(const WinArgs& a, int index) {
+  Item it;
+  const int rest = index / a.splits;
+  it.split = index - rest * a.splits;
+  const int heads = rest / a.blocks;
+  it.block = a.blocks - 1 - (rest - heads * a.blocks);   // the last positions of a causal call see the most keys: first
+  const int groups = a.H / a.pack;
+  it.b = heads / groups;
+  it.h0 = (heads - it.b * groups) * a.pack;
+  it.hkv = it.h0 / a.share;
+  return it;
+}
+
 // What a CTA reads: the same numbers in every role.
 struct Span {
-  int n;                 // keys of this sequence
-  int p_min, p_max;      // positions of its rows
-  int sink_tiles, win0;  // steps 0..sink_tiles-1 are tiles 0.., the others win0..
-  int step0, steps;      // this CTA's share of the steps
+  int n;                     // keys of this sequence
+  int lo_full, hi_full;      // every row sees every key of [lo_full, hi_full] (and those before `sinks`)
+  int steps;                 // this CTA's share of the key tiles
+  int first, sink_steps, win;   // step j is tile first + j while j < sink_steps, win + j from there
 };
 
 __device__ __forceinline__ int sequence_keys(const int* lengths, int b, int Sk) {
@@ -115,35 +145,34 @@ __device__ __forceinline__ int first_key(int p, int left) {
   return left < 0 ? 0 : max((int)max((int64_t)p - left, (int64_t)-1), 0);
 }
 
-template <int ROWS>
-__device__ __forceinline__ Span make_span(const WinArgs& a, int row0, int b, int split) {
+// positions: of the item's rows, the first at pos0
+__device__ __forceinline__ Span make_span(const WinArgs& a, int pos0, int positions, int b, int split) {
   Span s;
   s.n = sequence_keys(a.lengths, b, a.Sk);
-  const int last_row = min(row0 + ROWS, a.rows) - 1;
-  s.p_min = row0 / a.share + s.n - a.Sq;
-  s.p_max = last_row / a.share + s.n - a.Sq;
-  const int end = last_key(s.p_max, a.right, s.n) + 1;           // <= 0: nothing is visible
-  const int begin = first_key(s.p_min, a.left);
-  int total = 0;
-  s.sink_tiles = s.win0 = 0;
+  const int p_min = pos0 + s.n - a.Sq;
+  const int p_max = min(pos0 + positions, a.Sq) - 1 + s.n - a.Sq;
+  s.lo_full = first_key(p_max, a.left);
+  s.hi_full = last_key(p_min, a.right, s.n);
+  const int end = last_key(p_max, a.right, s.n) + 1;             // <= 0: nothing is visible
+  int total = 0, sink_tiles = 0, win0 = 0;
   if (end > 0) {
-    s.win0 = begin / BLOCK_N;
-    s.sink_tiles = min((min(a.sinks, end) + BLOCK_N - 1) / BLOCK_N, s.win0);
-    total = s.sink_tiles + max((end + BLOCK_N - 1) / BLOCK_N - s.win0, 0);
+    win0 = first_key(p_min, a.left) / BLOCK_N;
+    sink_tiles = min((min(a.sinks, end) + BLOCK_N - 1) / BLOCK_N, win0);
+    total = sink_tiles + max((end + BLOCK_N - 1) / BLOCK_N - win0, 0);
   }
-  s.step0 = (int)((int64_t)total * split / a.splits);
-  s.steps = (int)((int64_t)total * (split + 1) / a.splits) - s.step0;
+  s.first = (int)((int64_t)total * split / a.splits);
+  s.steps = (int)((int64_t)total * (split + 1) / a.splits) - s.first;
+  s.sink_steps = sink_tiles - s.first;
+  s.win = win0 - sink_tiles + s.first;
   return s;
 }
 // first key of the CTA's step j
 __device__ __forceinline__ int step_key(const Span& s, int j) {
-  const int g = s.step0 + j;
-  return (g < s.sink_tiles ? g : s.win0 + g - s.sink_tiles) * BLOCK_N;
+  return ((j < s.sink_steps ? s.first : s.win) + j) * BLOCK_N;
 }
 // some row of the CTA does not see the whole tile
 __device__ __forceinline__ bool is_mixed(const WinArgs& a, const Span& s, int key0) {
-  return key0 + BLOCK_N - 1 > last_key(s.p_min, a.right, s.n) ||
-         (key0 < first_key(s.p_max, a.left) && key0 + BLOCK_N > a.sinks);
+  return key0 + BLOCK_N - 1 > s.hi_full || (key0 < s.lo_full && key0 + BLOCK_N > a.sinks);
 }
 __device__ __forceinline__ bool sees_any(const WinArgs& a, int p, int n) {
   const int last = last_key(p, a.right, n);
@@ -163,6 +192,14 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
     tma_load_4d(dst, map, bar, 0, row0, h, b);
     tma_load_4d(dst + HALF_BYTES, map, bar, 64, row0, h, b);
   }
+}
+
+// one tile of Q: positions pos0.. of `pack` heads (positions past the sequence arrive as zeros)
+__device__ __forceinline__ void load_q(uint32_t dst, const CUtensorMap* map, uint32_t bar, const WinArgs& a, int pos0,
+                                       int h0, int b) {
+  mbar_expect_tx(bar, (uint32_t)(a.pack * a.tile_pos) * HEAD_DIM * 2);
+  tma_load_4d(dst, map, bar, 0, h0, pos0, b);
+  tma_load_4d(dst + HALF_BYTES, map, bar, 64, h0, pos0, b);
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -250,12 +287,525 @@ struct PartSum {
   }
 };
 
-// FEW: at most 128 rows per key head; the two tiles are two streams over the same rows.
-template <bool FEW>
+// What one softmax thread knows of its row.
+struct Row {
+  int key_first, key_last;             // visible: these, those between and the first keys
+  bool live;                           // a row of the tensor: others hold anything and must not cause a rescaling
+  float top = -INFINITY, sum = 0.f;    // running maximum of the raw scores, sum of the exponentials
+  __device__ __forceinline__ Row(const WinArgs& a, int position, int n, bool exists)
+      : key_first(first_key(position, a.left)), key_last(last_key(position, a.right, n)), live(exists) {}
+};
+
+// One step of one tile: scores from tensor memory -> masked -> P in their place, O rescaled if the
+// maximum grew (`rescale` is false on the row's first step, when O holds nothing).  `publish(part)`
+// hands a half of P to the MMA issuer.
+template <class Publish>
+__device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t o_tmem, float sl2, int sinks, int key0,
+                                             bool rescale, int lane, Publish publish) {
+  uint32_t s[128];
+#pragma unroll
+  for (int c = 0; c < 128; c += 32) tmem_ld_32x32b_x32(s_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
+  tmem_wait_ld();
+  {
+    // visible columns: [first, last] and those before `sink`
+    const int last = row.key_last - key0, first = row.key_first - key0, sink = sinks - key0;
+    if (__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N))) {
+      // a bit per visible column, 32 at a time: testing constant bits of a word costs a third of
+      // three comparisons per score
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t seen = columns_below(last + 1 - 32 * w) & (~columns_below(first - 32 * w) | columns_below(sink - 32 * w));
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!(seen & (1u << i))) s[32 * w + i] = 0xff800000u;   // -inf
+      }
+    }
+  }
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 128; c += 2)
+    mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+  const float m_row = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  const bool raise = row.live && (m_row - row.top) * sl2 > 8.0f;   // false while both are -inf (NaN)
+  float alpha = 1.0f;
+  if (raise) {
+    alpha = ex2_approx((row.top - m_row) * sl2);
+    row.top = m_row;
+    row.sum *= alpha;
+  }
+  __syncwarp();
+  if (rescale && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 16) {
+      uint32_t o[16];
+      tmem_ld_32x32b_x16(o_tmem + c, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      tmem_st_32x32b_x16(o_tmem + c, o);
+    }
+  }
+  // a row that has seen nothing yet has only -inf scores: exp2(-inf - 0) = 0
+  const float neg_ms = row.top == -INFINITY ? 0.0f : -row.top * sl2;
+  const uint64_t sl2x2 = pack2(sl2, sl2), nmsx2 = pack2(neg_ms, neg_ms);
+  uint64_t sm2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t p[8];
+    exp_chunk(&s[16 * q], p, sl2x2, nmsx2, sm2);
+    tmem_st_32x32b_x8(s_tmem + 8 * q, p);   // P takes the first half of S
+    if ((q + 1) % 4 == 0) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) publish(q / 4);
+    }
+  }
+  float a0, a1, b0, b1, c0, c1, d0, d1;
+  unpack2(sm2[0], a0, a1);
+  unpack2(sm2[1], b0, b1);
+  unpack2(sm2[2], c0, c1);
+  unpack2(sm2[3], d0, d1);
+  row.sum += ((a0 + a1) + (b0 + b1)) + ((c0 + c1) + (d0 + d1));
+}
+static_assert(P_PARTS == 2, "P is published in halves");
+
+// Adds the non-finite values that the fix warps took out of the mixed tiles to 32 columns of a row that
+// sees them: the steps first, first + stride, ... of the item.
+__device__ __forceinline__ void add_nonfinite(const WinArgs& a, const Span& span, const Row& row, int first, int stride,
+                                              int steps, int hkv, int b, int c, uint32_t (&o)[32]) {
+  for (int u = first; u < steps; u += stride) {
+    const int key0 = step_key(span, u);
+    if (!is_mixed(a, span, key0)) continue;
+    for (int j = key0; j < key0 + BLOCK_N && j <= row.key_last; ++j) {
+      if (j < row.key_first && j >= a.sinks) continue;
+      const __nv_bfloat16* src = a.v + b * a.v_b + hkv * a.v_h + (int64_t)j * a.v_s + c;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float x = __bfloat162float(src[i]);
+        if (!(fabsf(x) <= 3.4e38f)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+      }
+    }
+  }
+}
+__device__ __forceinline__ void store_f32(float* dst, const uint32_t (&o)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+}
+__device__ __forceinline__ void store_bf16(__nv_bfloat16* dst, const uint32_t (&o)[32], float inv) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 w;
+    w.x = pack_bf16x2_rn(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+    w.y = pack_bf16x2_rn(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+    w.z = pack_bf16x2_rn(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+    w.w = pack_bf16x2_rn(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+    reinterpret_cast<uint4*>(dst)[i] = w;
+  }
+}
+
+// The join of a cluster's parts: every CTA holds (slot) rows in shared memory; a warp takes a row, a
+// lane four columns, and the rows go round the CTAs.  PARTS slots of a CTA belong to one row.
+// row_of(r) gives the position and head of row r.
+template <class L, int PARTS, class RowOf>
+__device__ __forceinline__ void join_cluster(const WinArgs& a, uint32_t sbase, int warp, int lane, int split, int b, int n,
+                                             int nrows, RowOf row_of) {
+  for (int r = warp * a.splits + split; r < nrows; r += kSoftmaxWarps * a.splits) {
+    int pos, head;
+    if (!row_of(r, pos, head)) continue;
+    PartSum sum;
+    bool any_nan = false;
+    for (int p = 0; p < PARTS * a.splits; ++p) {
+      const float2 ml = ld_cluster_f2(map_to_cta(sbase + L::ML + (p % PARTS * BLOCK_M + r) * 8, p / PARTS));
+      sum.top = fmaxf(sum.top, ml.x);
+      any_nan |= ml.y != ml.y;
+    }
+    for (int p = 0; p < PARTS * a.splits; ++p) {
+      const int slot = p % PARTS * BLOCK_M + r, cta = p / PARTS;
+      sum.add(ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, cta)),
+              ld_cluster_f4(map_to_cta(sbase + (slot * L::PITCH + lane * 4) * 4, cta)));
+    }
+    const float inv = any_nan ? __uint_as_float(0x7fc00000u) : row_inverse(a, sum.l, pos + n - a.Sq, n);
+    reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Sq + pos) * a.H + head) * HEAD_DIM)[lane] = sum.row(inv);
+  }
+}
+
+// The work scheduler: a running CTA takes the place of one that has not been launched yet.
+__device__ __forceinline__ void ask_next(uint32_t answer, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+               "r"(bar)
+               : "memory");
+}
+// index of the block taken over, -1 when there was none left
+__device__ __forceinline__ int read_next(uint32_t answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(answer)
+      : "memory");
+  return got ? (int)x : -1;
+}
+
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ WinArgs args) {
+  using L = WinSmem<false>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::NUM);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // Set when a mixed tile held a non-finite value and never cleared: the path that it opens looks for
+  // itself and adds nothing where there is nothing.
+  volatile int* nonfinite = abort_flag + 1;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int idx) -> uint32_t { return bar0 + idx * 8; };
+  auto wait = [&](int idx, uint32_t parity) -> bool { return mbar_wait(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const bool more = args.join == 0;   // a cluster's CTAs do one item
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::NUM; ++i) {
+      int count = 1;
+      if (i == L::OE || i == L::OE + 1 || (i >= L::PF && i < L::KF)) count = 4;   // the tile's four warps
+      if (i == L::NE || i == L::NE + 1) count = kSoftmaxWarps + 4;                // every warp that asks
+      if (i >= L::VE && i < L::VC) count = 1 + kFixThreads / 32;                  // MMAs done, looked through
+      if (i >= L::VC) count = kFixThreads;
+      mbar_init(bar(i), count);
+    }
+    *abort_flag = 0;
+    *nonfinite = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  const int tile_rows = args.tile_pos * args.pack;
+  if (tile_rows < BLOCK_M) {   // rows that no load of Q reaches: zeros, like those past the sequence
+    for (int i = threadIdx.x; i < 4 * (BLOCK_M - tile_rows) * 8; i += NUM_THREADS)
+      sts128(sbase + L::Q + (i & 3) * HALF_BYTES + (tile_rows + (i >> 5)) * 128 + ((i >> 2) & 7) * 16, make_uint4(0, 0, 0, 0));
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int item_pos = 2 * args.tile_pos;
+
+  // The item after `fetch` others, or -1.  Called by whole warps (the loader by one lane) in step.
+  auto next_item = [&](int fetch) -> int {
+    if (!more) return -1;
+    const int slot = fetch & 1;
+    if (!wait(L::NF + slot, fetch >> 1)) return -1;
+    const int next = read_next(sbase + L::NEXT + slot * 16);
+    fence_proxy_async_smem();   // read before the scheduler writes there again
+    return next;
+  };
+
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TILE_REGS_SERVICE));
+    if (warp == kLoadWarp) {
+      if (lane == 0) {
+        int index = blockIdx.x, g = 0, full_items = 0;
+        bool ok = true;
+        for (int fetch = 0; ok && index >= 0; ++fetch) {
+          const Item it = decode_item(args, index);
+          const int pos0 = it.block * item_pos;
+          const Span span = make_span(args, pos0, item_pos, it.b, it.split);
+          // The next item is asked for with two steps to go: early enough to load it without a pause,
+          // late enough that no CTA holds an item back while another has nothing to do.
+          auto ask = [&]() -> bool {
+            const int slot = fetch & 1;
+            if (!wait(L::NE + slot, (fetch >> 1) ^ 1)) return false;   // its last answer has been read by every warp
+            ask_next(sbase + L::NEXT + slot * 16, bar(L::NF + slot));
+            return true;
+          };
+          if (more && span.steps == 0) ok = ask();
+          for (int j = 0; ok && j < span.steps; ++j) {
+            const int st = (g + j) & 1;
+            const uint32_t use = (uint32_t)(g + j) >> 1;
+            const int key0 = step_key(span, j);
+            if (!(ok = wait(L::KE + st, use ^ 1))) break;
+            if (more && j == max(0, span.steps - 2) && !(ok = ask())) break;
+            load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), key0, it.hkv, it.b, args.k_swap);
+            if (j == 0) {
+              // Q once the last item's scores are all computed
+              if (!(ok = wait(L::QE, full_items ^ 1))) break;
+              for (int t = 0; t < 2; ++t) load_q(sbase + L::Q + t * TILE_BYTES, &tmap_q, bar(L::QF + t), args, pos0 + t * args.tile_pos, it.h0, it.b);
+            }
+            if (!(ok = wait(L::VE + st, use ^ 1))) break;
+            load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), key0, it.hkv, it.b, args.v_swap);
+          }
+          g += span.steps;
+          full_items += span.steps > 0;
+          if (!ok) break;
+          index = next_item(fetch);
+          if (more) mbar_arrive(bar(L::NE + (fetch & 1)));
+        }
+      }
+    } else if (warp >= kFixWarp) {
+      const int ft = threadIdx.x - kFixWarp * 32;
+      int index = blockIdx.x, g = 0;
+      bool ok = true;
+      for (int fetch = 0; ok && index >= 0; ++fetch) {
+        const Item it = decode_item(args, index);
+        const Span span = make_span(args, it.block * item_pos, item_pos, it.b, it.split);
+        // every step is waited for and released, mixed or not: these warps can neither run ahead of
+        // the ring by a whole phase nor fall behind it by one
+        for (int j = 0; ok && j < span.steps; ++j) {
+          const int key0 = step_key(span, j);
+          const int st = (g + j) & 1;
+          if (!(ok = wait(L::VF + st, (uint32_t)(g + j) >> 1))) break;
+          if (is_mixed(args, span, key0)) {
+            if (clean_values(sbase + L::V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
+            fence_proxy_async_smem();
+            mbar_arrive(bar(L::VC + st));
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(L::VE + st));
+        }
+        g += span.steps;
+        if (!ok) break;
+        index = next_item(fetch);
+        __syncwarp();
+        if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
+      }
+    } else {
+      const bool leader = elect_one() != 0;
+      const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // tile 1: 128 columns on
+      const uint32_t q0 = desc_lo(sbase + L::Q, 16);
+      const uint32_t k0 = desc_lo(sbase + L::K, 16);
+      const uint32_t v0 = desc_lo(sbase + L::V, HALF_BYTES);
+      constexpr uint32_t TILE_UNITS = TILE_BYTES >> 4;
+      uint32_t clean_phase = 0;   // bit per stage
+      int index = blockIdx.x, g = 0, full_items = 0;
+      bool ok = true;
+      // S of tile t = Q . K^T of the stage's keys
+      auto issue_qk = [&](int t, int st) {
+        if (leader) mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + t * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
+        if (leader) tc_commit(bar(L::SF + t));
+      };
+      // O of tile t += P . V, each half of P as soon as it is published; `step` counts over all items
+      auto issue_pv = [&](int t, int step, bool first) -> bool {
+        const int st = step & 1;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!wait(L::PF + 2 * part + t, step)) return false;
+          tc_fence_after();
+          if (leader) {
+            if (part == 0)
+              mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, first ? 0u : 1u);
+            else
+              mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
+          }
+        }
+        return true;
+      };
+      for (int fetch = 0; ok && index >= 0; ++fetch) {
+        const Item it = decode_item(args, index);
+        const Span span = make_span(args, it.block * item_pos, item_pos, it.b, it.split);
+        const int steps = span.steps;
+        // the step's values are there, and cleared if the tile is mixed
+        auto wait_v = [&](int j) -> bool {
+          const int st = (g + j) & 1;
+          if (!wait(L::VF + st, (uint32_t)(g + j) >> 1)) return false;
+          if (is_mixed(args, span, step_key(span, j))) {
+            if (!wait(L::VC + st, clean_phase >> st)) return false;
+            clean_phase ^= 1u << st;
+          }
+          return true;
+        };
+        auto wait_k = [&](int j) -> bool {
+          if (!wait(L::KF + ((g + j) & 1), (uint32_t)(g + j) >> 1)) return false;
+          tc_fence_after();
+          return true;
+        };
+        if (steps > 0) {
+          if (!(ok = wait_k(0) && wait(L::QF, full_items))) break;
+          tc_fence_after();
+          issue_qk(0, g & 1);
+          if (!(ok = wait(L::QF + 1, full_items))) break;
+          tc_fence_after();
+          issue_qk(1, g & 1);
+          if (leader) tc_commit(bar(L::KE + (g & 1)));
+          if (steps == 1 && leader) tc_commit(bar(L::QE));
+          // the softmax warps have read the last item's O
+          if (full_items > 0 && !(ok = wait(L::OE, full_items - 1) && wait(L::OE + 1, full_items - 1))) break;
+          if (!(ok = wait_v(0))) break;
+          for (int j = 0; j < steps; ++j) {
+            const int st = (g + j) & 1;
+            const bool last = j + 1 == steps;
+            if (!(ok = issue_pv(0, g + j, j == 0))) break;
+            if (last) {
+              if (leader) tc_commit(bar(L::OF));
+            } else {
+              if (!(ok = wait_k(j + 1))) break;
+              issue_qk(0, st ^ 1);
+            }
+            if (!(ok = issue_pv(1, g + j, j == 0))) break;
+            if (leader) tc_commit(bar(L::VE + st));
+            if (last) {
+              if (leader) tc_commit(bar(L::OF + 1));
+            } else {
+              // the next step's values, waited for while this step's MMAs are still queued
+              if (!(ok = wait_v(j + 1))) break;
+              issue_qk(1, st ^ 1);
+              if (leader) tc_commit(bar(L::KE + (st ^ 1)));
+              if (j + 2 == steps && leader) tc_commit(bar(L::QE));
+            }
+          }
+          if (!ok) break;
+          g += steps;
+          ++full_items;
+        }
+        index = next_item(fetch);
+        __syncwarp();
+        if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
+      }
+    }
+    if (args.join) {   // the softmax warps' two meetings
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TILE_REGS_SOFTMAX));
+    const int t = warp >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int row_pos = min(r, tile_rows - 1) / args.pack;          // position within the tile, and head
+    const int row_head = min(r, tile_rows - 1) - row_pos * args.pack;
+    const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem_base + COL_S0 + t * 128 + lane_sel;
+    const uint32_t o_tmem = tmem_base + COL_O0 + t * 128 + lane_sel;
+    int index = blockIdx.x, g = 0, full_items = 0;
+    bool ok = true;
+    for (int fetch = 0; index >= 0; ++fetch) {
+      const Item it = decode_item(args, index);
+      const int pos0 = it.block * item_pos;
+      const Span span = make_span(args, pos0, item_pos, it.b, it.split);
+      const int steps = span.steps;
+      const int pos = pos0 + t * args.tile_pos + row_pos;
+      const bool row_ok = r < tile_rows && pos < args.Sq;
+      const bool warp_ok = __any_sync(0xffffffffu, row_ok);
+      Row row(args, min(pos, args.Sq - 1) + span.n - args.Sq, span.n, row_ok);
+      for (int u = 0; u < steps; ++u) {
+        if (ok) ok = wait(L::SF + t, g + u);
+        tc_fence_after();
+        if (!warp_ok) {   // none of the warp's rows exist: whatever P holds there goes nowhere
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar(L::PF + t));
+            mbar_arrive(bar(L::PF + 2 + t));
+          }
+          continue;
+        }
+        softmax_step(row, s_tmem, o_tmem, args.scale_log2, args.sinks, step_key(span, u), u != 0, lane,
+                     [&](int part) { mbar_arrive(bar(L::PF + 2 * part + t)); });
+      }
+      g += steps;
+      if (ok && steps > 0) ok = wait(L::OF + t, full_items);
+      // the rows to join take the operands' place: no MMA of the other tile may still read them
+      if (ok && args.join && steps > 0) ok = wait(L::OF + (t ^ 1), full_items);
+      tc_fence_after();
+      const bool parts = args.part_o != nullptr;
+      const int64_t out_row = ((int64_t)it.b * args.Sq + min(pos, args.Sq - 1)) * args.H + it.h0 + row_head;
+      if (ok && warp_ok) {
+        const float inv = row.sum != row.sum ? 1.0f : row_inverse(args, row.sum, min(pos, args.Sq - 1) + span.n - args.Sq, span.n);
+        const int slot = t * BLOCK_M + r;
+        if (row_ok) {
+          const float2 ml = make_float2(row.top * args.scale_log2, row.sum);
+          if (args.join)
+            reinterpret_cast<float2*>(smem + L::ML)[slot] = ml;
+          else if (parts)
+            args.part_ml[it.split * args.total_rows + out_row] = ml;
+        }
+        __syncwarp();
+        const bool fix = *nonfinite != 0;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld_32x32b_x32(o_tmem + c, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (c == 96 && steps > 0) {   // O is in registers: the next item's may be written
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::OE + t));
+          }
+          if (fix && row_ok) add_nonfinite(args, span, row, 0, 1, steps, it.hkv, it.b, c, o);
+          if (row_ok) {
+            if (args.join)
+              store_f32(reinterpret_cast<float*>(smem) + slot * L::PITCH + c, o);
+            else if (parts)
+              store_f32(args.part_o + (it.split * args.total_rows + out_row) * HEAD_DIM + c, o);
+            else
+              store_bf16(args.out + out_row * HEAD_DIM + c, o, inv);
+          }
+          __syncwarp();   // the next columns are loaded by the whole warp
+        }
+      } else if (steps > 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::OE + t));
+      }
+      full_items += steps > 0;
+      if (args.join) {
+        __syncwarp();
+        cluster_sync_all();   // every CTA's rows are in its shared memory
+        join_cluster<L, 1>(args, sbase, warp, lane, it.split, it.b, span.n, 2 * BLOCK_M, [&](int rr, int& p, int& h) {
+          const int tt = rr / BLOCK_M, in = rr % BLOCK_M;
+          const int rp = in / args.pack;
+          p = pos0 + tt * args.tile_pos + rp;
+          h = it.h0 + in - rp * args.pack;
+          return in < tile_rows && p < args.Sq;
+        });
+        __syncwarp();
+        cluster_sync_all();   // no CTA retires while another reads its rows
+      }
+      index = ok ? next_item(fetch) : -1;
+      __syncwarp();
+      if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag != 0) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 200000) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// At most 128 rows per key head: the two tiles are two streams over the same rows.
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                   const __grid_constant__ WinArgs args) {
-  using L = WinSmem<FEW>;
+  using L = WinSmem<true>;
   constexpr int STAGES = L::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -267,19 +817,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int idx) -> uint32_t { return bar0 + idx * 8; };
+  auto wait = [&](int idx, uint32_t parity) -> bool { return mbar_wait(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  constexpr int CTA_ROWS = FEW ? BLOCK_M : 2 * BLOCK_M;
-  // the last rows of a causal call see the most keys: they start first
-  const int block = gridDim.x / args.splits - 1 - blockIdx.x / args.splits;
-  const int split = blockIdx.x % args.splits;
-  const int hkv = blockIdx.y, b = blockIdx.z;
-  const int row0 = block * CTA_ROWS;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NUM; ++i) {
       int count = 1;
-      if (i < L::SF || (i >= L::PF && i < L::KF)) count = 4;             // the tile's four warps
+      if (i == L::QF || (i >= L::PF && i < L::KF)) count = 4;            // the tile's four warps
       if (i >= L::VE && i < L::VC) count = 1 + kFixThreads / 32;         // MMAs done, looked through
       if (i >= L::VC) count = kFixThreads;
       mbar_init(bar(i), count);
@@ -298,44 +843,37 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const Span span = make_span<CTA_ROWS>(args, row0, b, split);
+  const Item it = decode_item(args, blockIdx.x);
+  const Span span = make_span(args, 0, args.Sq, it.b, it.split);
   const int steps = span.steps;
 
   if (warp >= kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WIN_REGS_SERVICE));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS_SERVICE));
     if (warp == kLoadWarp) {
       if (lane == 0) {
         auto load_k = [&](int j) -> bool {
           const int st = j % STAGES;
-          if (!mbar_wait(bar(L::KE + st), ((j / STAGES) & 1) ^ 1, abort_flag, kStatusFlashTimeout)) return false;
-          load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), step_key(span, j), hkv, b, args.k_swap);
+          if (!wait(L::KE + st, (j / STAGES) ^ 1)) return false;
+          load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), step_key(span, j), it.hkv, it.b, args.k_swap);
           return true;
         };
         auto load_v = [&](int j) -> bool {
           const int st = j % STAGES;
-          if (!mbar_wait(bar(L::VE + st), ((j / STAGES) & 1) ^ 1, abort_flag, kStatusFlashTimeout)) return false;
-          load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), step_key(span, j), hkv, b, args.v_swap);
+          if (!wait(L::VE + st, (j / STAGES) ^ 1)) return false;
+          load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), step_key(span, j), it.hkv, it.b, args.v_swap);
           return true;
         };
-        // In the few-row form a step's K is free long before its V (the streams' MMAs alternate), so
-        // K runs a step ahead: behind V it would wait for the other stream's product as well.
-        bool ok = steps == 0 || !FEW || load_k(0);
-        for (int j = 0; ok && j < steps; ++j) {
-          if constexpr (FEW)
-            ok = j + 1 >= steps || load_k(j + 1);
-          else
-            ok = load_k(j);
-          ok = ok && load_v(j);
-        }
+        // A step's K is free long before its V (the streams' MMAs alternate), so K runs a step ahead:
+        // behind V it would wait for the other stream's product as well.
+        bool ok = steps == 0 || load_k(0);
+        for (int j = 0; ok && j < steps; ++j) ok = (j + 1 >= steps || load_k(j + 1)) && load_v(j);
       }
     } else if (warp >= kFixWarp) {
       const int ft = threadIdx.x - kFixWarp * 32;
-      // every step is waited for and released, mixed or not: these warps can neither run ahead of
-      // the ring by a whole phase nor fall behind it by one
-      for (int j = 0; j < steps; ++j) {
+      for (int j = 0; j < steps; ++j) {   // every step, as in window_tile_kernel
         const int key0 = step_key(span, j);
         const int st = j % STAGES;
-        if (!mbar_wait(bar(L::VF + st), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) break;
+        if (!wait(L::VF + st, j / STAGES)) break;
         if (is_mixed(args, span, key0)) {
           if (clean_values(sbase + L::V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
           fence_proxy_async_smem();
@@ -344,105 +882,47 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L::VE + st));
       }
-    } else if (warp == kMmaWarp && steps > 0) {
+    } else if (steps > 0) {
       const bool leader = elect_one() != 0;
-      const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // tile 1: 128 columns on
+      const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // stream 1: 128 columns on
       const uint32_t q0 = desc_lo(sbase + L::Q, 16);
       const uint32_t k0 = desc_lo(sbase + L::K, 16);
       const uint32_t v0 = desc_lo(sbase + L::V, HALF_BYTES);
       constexpr uint32_t TILE_UNITS = TILE_BYTES >> 4;
       uint32_t clean_phase = 0;   // bit per stage
-      // S of tile t = Q . K^T of the stage's keys
-      auto issue_qk = [&](int t, int st) {
-        if (leader) mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + (FEW ? 0 : t) * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
-        if (leader) tc_commit(bar(L::SF + t));
-      };
-      auto wait_k = [&](int j) -> bool {
-        if (!mbar_wait(bar(L::KF + j % STAGES), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) return false;
+      // S of step j in stream j & 1
+      auto issue_qk = [&](int j) -> bool {
+        const int st = j % STAGES, t = j & 1;
+        if (!wait(L::KF + st, j / STAGES)) return false;
         tc_fence_after();
+        if (leader) {
+          mma_f16_ss_kmajor_x8(s0 + t * 128, q0, k0 + st * TILE_UNITS, kIdescQK);
+          tc_commit(bar(L::SF + t));
+          tc_commit(bar(L::KE + st));
+        }
         return true;
       };
-      // the step's values are there, and cleared if the tile is mixed
-      auto wait_v = [&](int j) -> bool {
-        const int st = j % STAGES;
-        if (!mbar_wait(bar(L::VF + st), (j / STAGES) & 1, abort_flag, kStatusFlashTimeout)) return false;
+      bool ok = wait(L::QF, 0) && issue_qk(0) && (steps == 1 || issue_qk(1));
+      for (int j = 0; ok && j < steps; ++j) {
+        const int st = j % STAGES, t = j & 1;
+        if (!(ok = wait(L::VF + st, j / STAGES))) break;
         if (is_mixed(args, span, step_key(span, j))) {
-          if (!mbar_wait(bar(L::VC + st), (clean_phase >> st) & 1, abort_flag, kStatusFlashTimeout)) return false;
+          if (!(ok = wait(L::VC + st, clean_phase >> st))) break;
           clean_phase ^= 1u << st;
         }
-        return true;
-      };
-      // O of tile t += P . V, each half of P as soon as it is published; `use` counts the tile's steps
-      auto issue_pv = [&](int t, int st, int use) -> bool {
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          if (!mbar_wait(bar(L::PF + 2 * part + t), use & 1, abort_flag, kStatusFlashTimeout)) return false;
-          tc_fence_after();
-          if (leader) {
-            if (part == 0)
-              mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, use != 0 ? 1u : 0u);
-            else
-              mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
-          }
+        if (!(ok = wait(L::PF + t, j >> 1))) break;
+        tc_fence_after();
+        if (leader) mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, j > 1 ? 1u : 0u);
+        if (!(ok = wait(L::PF + 2 + t, j >> 1))) break;
+        tc_fence_after();
+        if (leader) {
+          mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
+          tc_commit(bar(L::VE + st));
         }
-        return true;
-      };
-      static_assert(P_PARTS == 2, "P is published in halves");
-      bool ok = mbar_wait(bar(L::QF), 0, abort_flag, kStatusFlashTimeout) && wait_k(0);
-      if constexpr (FEW) {
-        // step j belongs to stream j & 1
-        if (ok) {
-          issue_qk(0, 0);
-          if (leader) tc_commit(bar(L::KE));
-        }
-        if (ok && steps > 1 && (ok = wait_k(1))) {
-          issue_qk(1, 1);
-          if (leader) tc_commit(bar(L::KE + 1));
-        }
-        for (int j = 0; ok && j < steps; ++j) {
-          const int t = j & 1;
-          if (!(ok = wait_v(j) && issue_pv(t, j % STAGES, j >> 1))) break;
-          if (leader) tc_commit(bar(L::VE + j % STAGES));
-          if (j + 2 < steps) {
-            if (!(ok = wait_k(j + 2))) break;
-            issue_qk(t, (j + 2) % STAGES);
-            if (leader) tc_commit(bar(L::KE + (j + 2) % STAGES));
-          } else {
-            if (leader) tc_commit(bar(L::OF + t));
-          }
-        }
-      } else {
-        if (ok) {
-          issue_qk(0, 0);
-          ok = mbar_wait(bar(L::QF + 1), 0, abort_flag, kStatusFlashTimeout);
-        }
-        if (ok) {
-          tc_fence_after();
-          issue_qk(1, 0);
-          if (leader) tc_commit(bar(L::KE));
-          ok = wait_v(0);
-        }
-        for (int j = 0; ok && j < steps; ++j) {
-          const int st = j & 1;
-          const bool last = j + 1 == steps;
-          if (!(ok = issue_pv(0, st, j))) break;
-          if (last) {
-            if (leader) tc_commit(bar(L::OF));
-          } else {
-            if (!(ok = wait_k(j + 1))) break;
-            issue_qk(0, st ^ 1);
-          }
-          if (!(ok = issue_pv(1, st, j))) break;
-          if (leader) tc_commit(bar(L::VE + st));
-          if (last) {
-            if (leader) tc_commit(bar(L::OF + 1));
-          } else {
-            // the next step's values, waited for while this step's MMAs are still queued
-            if (!(ok = wait_v(j + 1))) break;
-            issue_qk(1, st ^ 1);
-            if (leader) tc_commit(bar(L::KE + (st ^ 1)));
-          }
-        }
+        if (j + 2 < steps)
+          ok = issue_qk(j + 2);
+        else if (leader)
+          tc_commit(bar(L::OF + t));
       }
     }
     if (args.join) {   // the softmax warps' two meetings
@@ -451,52 +931,47 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       cluster_sync_all();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(B2_FLASH_REGS_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FEW_REGS_SOFTMAX));
     const int t = warp >> 2;
     const int quarter = warp & 3;
-    const int tile_row0 = row0 + (FEW ? 0 : t * BLOCK_M);
-    if (steps > 0 && (!FEW || t == 0)) {
-      // this tile's rows of Q: 16 lanes per row, all loads in flight before the first store
+    const int rows = args.Sq * args.pack;
+    if (steps > 0 && t == 0) {
+      // the rows of Q: 16 lanes per row, all loads in flight before the first store
       const int tid = threadIdx.x & 127, c16 = tid & 15;
       uint4 v[16];
 #pragma unroll
       for (int p = 0; p < 16; ++p) {
-        const int r = tile_row0 + p * 8 + (tid >> 4);
+        const int r = p * 8 + (tid >> 4);
         v[p] = make_uint4(0, 0, 0, 0);
-        if (r < args.rows) {
-          const int i = r / args.share, h = hkv * args.share + (r - i * args.share);
-          v[p] = ldg_stream(reinterpret_cast<const uint4*>(args.q + b * args.q_b + h * args.q_h + i * args.q_s) + c16);
+        if (r < rows) {
+          const int i = r / args.pack, h = it.h0 + r - i * args.pack;
+          v[p] = ldg_stream(reinterpret_cast<const uint4*>(args.q + it.b * args.q_b + h * args.q_h + i * args.q_s) + c16);
         }
       }
 #pragma unroll
       for (int p = 0; p < 16; ++p) {
         const int r = p * 8 + (tid >> 4);
-        sts128(sbase + L::Q + t * TILE_BYTES + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
+        sts128(sbase + L::Q + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::QF + t));
+      if (lane == 0) mbar_arrive(bar(L::QF));
     }
-    const int uses = FEW ? (steps + 1 - t) >> 1 : steps;   // steps of this tile (stream)
-    const int row = tile_row0 + quarter * 32 + lane;
-    const bool row_ok = row < args.rows;
-    const bool warp_ok = tile_row0 + quarter * 32 < args.rows;
-    const int my_row = min(row, args.rows - 1);
-    const int my_i = my_row / args.share;
-    const int p_row = my_i + span.n - args.Sq;
-    const int key_last = last_key(p_row, args.right, span.n);
-    const int key_first = first_key(p_row, args.left);
+    const int uses = (steps + 1 - t) >> 1;   // steps of this stream
+    const int r = quarter * 32 + lane;
+    const bool row_ok = r < rows;
+    const bool warp_ok = quarter * 32 < rows;
+    const int pos = min(r, rows - 1) / args.pack;
+    const int head = it.h0 + min(r, rows - 1) - pos * args.pack;
+    Row row(args, pos + span.n - args.Sq, span.n, row_ok);
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem_base + COL_S0 + t * 128 + lane_sel;
-    const uint32_t p_tmem = s_tmem;
     const uint32_t o_tmem = tmem_base + COL_O0 + t * 128 + lane_sel;
-    const float sl2 = args.scale_log2;
     bool ok = true;
-    float row_max = -INFINITY, row_sum = 0.f;
     for (int u = 0; u < uses; ++u) {
-      if (ok) ok = mbar_wait(bar(L::SF + t), u & 1, abort_flag, kStatusFlashTimeout);
+      if (ok) ok = wait(L::SF + t, u);
       tc_fence_after();
-      if (!warp_ok) {   // none of the warp's rows exist: whatever P holds there goes nowhere
+      if (!warp_ok) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -505,92 +980,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         }
         continue;
       }
-      uint32_t s[128];
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) tmem_ld_32x32b_x32(s_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
-      tmem_wait_ld();
-      {
-        // visible columns: [first, last] and those before `sink`
-        const int key0 = step_key(span, FEW ? 2 * u + t : u);
-        const int last = key_last - key0, first = key_first - key0, sink = args.sinks - key0;
-        if (__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N))) {
-          // a bit per visible column, 32 at a time: testing constant bits of a word costs a third of
-          // three comparisons per score
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t seen = columns_below(last + 1 - 32 * w) & (~columns_below(first - 32 * w) | columns_below(sink - 32 * w));
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen & (1u << i))) s[32 * w + i] = 0xff800000u;   // -inf
-          }
-        }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 128; c += 2)
-        mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-      const float m_row = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool raise = (m_row - row_max) * sl2 > 8.0f;   // false while both are -inf (NaN)
-      float alpha = 1.0f;
-      if (raise) {
-        alpha = ex2_approx((row_max - m_row) * sl2);
-        row_max = m_row;
-        row_sum *= alpha;
-      }
-      if (u != 0 && __any_sync(0xffffffffu, raise)) {
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 16) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(o_tmem + c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32b_x16(o_tmem + c, o);
-        }
-      }
-      // a row that has seen nothing yet has only -inf scores: exp2(-inf - 0) = 0
-      const float neg_ms = row_max == -INFINITY ? 0.0f : -row_max * sl2;
-      const uint64_t sl2x2 = pack2(sl2, sl2), nmsx2 = pack2(neg_ms, neg_ms);
-      uint64_t sm2[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        uint32_t p[8];
-        exp_chunk(&s[16 * q], p, sl2x2, nmsx2, sm2);
-        tmem_st_32x32b_x8(p_tmem + 8 * q, p);
-        if ((q + 1) % 4 == 0) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(L::PF + 2 * (q / 4) + t));
-        }
-      }
-      float a0, a1, b0, b1, c0, c1, d0, d1;
-      unpack2(sm2[0], a0, a1);
-      unpack2(sm2[1], b0, b1);
-      unpack2(sm2[2], c0, c1);
-      unpack2(sm2[3], d0, d1);
-      row_sum += ((a0 + a1) + (b0 + b1)) + ((c0 + c1) + (d0 + d1));
+      softmax_step(row, s_tmem, o_tmem, args.scale_log2, args.sinks, step_key(span, 2 * u + t), u != 0, lane,
+                   [&](int part) { mbar_arrive(bar(L::PF + 2 * part + t)); });
     }
-    if (ok && uses > 0) ok = mbar_wait(bar(L::OF + t), 0, abort_flag, kStatusFlashTimeout);
-    // the rows to join take the operands' place: no MMA of the other tile may still read them
-    const int other_uses = FEW ? (steps + t) >> 1 : steps;
-    if (ok && args.join && other_uses > 0) ok = mbar_wait(bar(L::OF + (t ^ 1)), 0, abort_flag, kStatusFlashTimeout);
-    // without parts the few-row form has a single step, which is stream 0's
+    if (ok && uses > 0) ok = wait(L::OF + t, 0);
+    // the rows to join take the operands' place: no MMA of the other stream may still read them
+    if (ok && args.join && ((steps + t) >> 1) > 0) ok = wait(L::OF + (t ^ 1), 0);
+    tc_fence_after();
     const bool parts = args.part_o != nullptr;
-    if (ok && warp_ok && !(FEW && t == 1 && !parts && !args.join)) {
-      tc_fence_after();
-      const int h = hkv * args.share + (my_row - my_i * args.share);
-      const int64_t out_row = ((int64_t)b * args.Sq + my_i) * args.H + h;
-      const int part = FEW ? 2 * split + t : split;
-      const float inv = parts || args.join || row_sum != row_sum ? 1.0f : row_inverse(args, row_sum, p_row, span.n);
-      const int slot = t * BLOCK_M + quarter * 32 + lane;
+    // with nothing to join there is a single step, which is stream 0's
+    if (ok && warp_ok && (t == 0 || parts || args.join)) {
+      const int64_t out_row = ((int64_t)it.b * args.Sq + pos) * args.H + head;
+      const int64_t part_row = (2 * it.split + t) * args.total_rows + out_row;
+      const float inv = row.sum != row.sum ? 1.0f : row_inverse(args, row.sum, pos + span.n - args.Sq, span.n);
+      const int slot = t * BLOCK_M + r;
       if (row_ok) {
-        const float2 ml = make_float2(row_max * sl2, row_sum);
+        const float2 ml = make_float2(row.top * args.scale_log2, row.sum);
         if (args.join)
           reinterpret_cast<float2*>(smem + L::ML)[slot] = ml;
         else if (parts)
-          args.part_ml[part * args.total_rows + out_row] = ml;
+          args.part_ml[part_row] = ml;
       }
+      __syncwarp();
       const bool fix = *nonfinite != 0;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
@@ -602,66 +1013,26 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (fix && row_ok) {
-          for (int u = 0; u < uses; ++u) {
-            const int key0 = step_key(span, FEW ? 2 * u + t : u);
-            if (!is_mixed(args, span, key0)) continue;
-            for (int j = key0; j < key0 + BLOCK_N && j <= key_last; ++j) {
-              if (j < key_first && j >= args.sinks) continue;
-              const __nv_bfloat16* src = args.v + b * args.v_b + hkv * args.v_h + (int64_t)j * args.v_s + c;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float x = __bfloat162float(src[i]);
-                if (!(fabsf(x) <= 3.4e38f)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
-              }
-            }
-          }
+        if (fix && row_ok) add_nonfinite(args, span, row, t, 2, steps, it.hkv, it.b, c, o);
+        if (row_ok) {
+          if (args.join)
+            store_f32(reinterpret_cast<float*>(smem) + slot * L::PITCH + c, o);
+          else if (parts)
+            store_f32(args.part_o + part_row * HEAD_DIM + c, o);
+          else
+            store_bf16(args.out + out_row * HEAD_DIM + c, o, inv);
         }
-        if (!row_ok) continue;
-        if (parts || args.join) {
-          float* dst = args.join ? reinterpret_cast<float*>(smem) + slot * L::PITCH + c
-                                 : args.part_o + (part * args.total_rows + out_row) * HEAD_DIM + c;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(args.out + out_row * HEAD_DIM + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 w;
-            w.x = pack_bf16x2_rn(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-            w.y = pack_bf16x2_rn(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-            w.z = pack_bf16x2_rn(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-            w.w = pack_bf16x2_rn(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-            dst[i] = w;
-          }
-        }
+        __syncwarp();   // the next columns are loaded by the whole warp
       }
     }
     if (args.join) {
       __syncwarp();
       cluster_sync_all();   // every CTA's rows are in its shared memory
-      // a warp takes a row, a lane four columns; the rows go round the cluster's CTAs
-      const int nrows = min(CTA_ROWS, args.rows - row0);
-      for (int r = warp * args.splits + split; r < nrows; r += kSoftmaxWarps * args.splits) {
-        PartSum sum;
-        bool any_nan = false;
-        for (int p = 0; p < (FEW ? 2 : 1) * args.splits; ++p) {
-          const int slot = FEW ? (p & 1) * BLOCK_M + r : r;
-          const float2 ml = ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, FEW ? p >> 1 : p));
-          sum.top = fmaxf(sum.top, ml.x);
-          any_nan |= ml.y != ml.y;
-        }
-        for (int p = 0; p < (FEW ? 2 : 1) * args.splits; ++p) {
-          const int slot = FEW ? (p & 1) * BLOCK_M + r : r;
-          const int cta = FEW ? p >> 1 : p;
-          sum.add(ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, cta)),
-                  ld_cluster_f4(map_to_cta(sbase + (slot * L::PITCH + lane * 4) * 4, cta)));
-        }
-        const int i = (row0 + r) / args.share, h = hkv * args.share + (row0 + r) % args.share;
-        const float inv = any_nan ? __uint_as_float(0x7fc00000u) : row_inverse(args, sum.l, i + span.n - args.Sq, span.n);
-        reinterpret_cast<uint2*>(args.out + (((int64_t)b * args.Sq + i) * args.H + h) * HEAD_DIM)[lane] = sum.row(inv);
-      }
+      join_cluster<L, 2>(args, sbase, warp, lane, it.split, it.b, span.n, rows, [&](int rr, int& p, int& h) {
+        p = rr / args.pack;
+        h = it.h0 + rr - p * args.pack;
+        return true;
+      });
       __syncwarp();
       cluster_sync_all();   // no CTA retires while another reads its rows
     }
@@ -710,6 +1081,7 @@ window_join_kernel(const WinArgs args, int parts) {
 // How a call is laid over the GPU: few-row form or not, splits of the key sequence, parts to join.
 struct WinPlan {
   bool few, join;
+  int pack, tile_pos;          // heads per row group, positions per tile
   int blocks, splits, parts;   // parts: to be joined by window_join_kernel (1: none)
 };
 WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks) {
@@ -717,11 +1089,20 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
   const int share = H / Hkv;
   const int64_t rows = (int64_t)Sq * share;
   p.few = rows <= BLOCK_M;
-  const int cta_rows = p.few ? BLOCK_M : 2 * BLOCK_M;
-  p.blocks = (int)((rows + cta_rows - 1) / cta_rows);
-  // the most 128-key steps that a CTA can have: its rows' positions, the window around them, the
-  // first keys; one more for a window that starts inside a tile
-  const int64_t positions = min((int64_t)Sq, (int64_t)cta_rows / share + 2);
+  // Heads per row group: as many of those that share a key head as fill seven eighths of a tile's 128
+  // rows (fewer positions per item see fewer keys in vain: 2 x 24 heads x 4099, three to a key
+  // head, window 1023: 126 rows in threes 158 us, 128 rows of one head 180 us).
+  p.pack = share;
+  if (!p.few) {
+    p.pack = 1;
+    for (int d = 2; d <= share && d <= BLOCK_M; ++d)
+      if (share % d == 0 && BLOCK_M / d * d >= 112) p.pack = d;
+  }
+  p.tile_pos = p.few ? Sq : BLOCK_M / p.pack;
+  p.blocks = p.few ? 1 : (Sq + 2 * p.tile_pos - 1) / (2 * p.tile_pos);
+  // the most 128-key steps that a CTA can have: its positions, the window around them, the first
+  // keys; one more for a window that starts inside a tile
+  const int64_t positions = min((int64_t)Sq, (int64_t)(p.few ? 1 : 2) * p.tile_pos);
   int64_t keys = Sk;
   if (left >= 0 && right >= 0) keys = min(keys, (int64_t)left + right + positions);
   int64_t steps = (keys + BLOCK_N - 1) / BLOCK_N + (keys < Sk ? 1 : 0);
@@ -735,7 +1116,7 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
   // and back.  For 24 heads' single tokens over 8192 keys: 65.6 us unsplit, 32.8 in clusters of four,
   // 35.8 in four parts through memory.
   constexpr int kSlots[kMaxCluster + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
-  const int64_t ctas = (int64_t)p.blocks * Hkv * B;
+  const int64_t ctas = (int64_t)p.blocks * (H / p.pack) * B;
   double best = 1e30;
   p.splits = 1;
   p.join = false;
@@ -746,7 +1127,7 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
     const double step = p.few ? (running * 0.0109 > 0.83 ? running * 0.0109 : 0.83) : 1.85;
     double cost = rounds * ((double)steps / s * step + (p.few ? 8.0 : 5.0));
     if (cluster && (s > 1 || p.few)) cost += p.few ? 1.0 : 7.0 * rounds;
-    if (!cluster) cost += 6.0 + 2.1e-4 * (double)(rows * Hkv * B) * s * (p.few ? 2 : 1);
+    if (!cluster) cost += 6.0 + 2.1e-4 * (double)((int64_t)Sq * H * B) * s * (p.few ? 2 : 1);
     if (cost < best) {
       best = cost;
       p.splits = s;
@@ -763,6 +1144,21 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
   return p;
 }
 
+// Q as (channel, head, position, batch): a box is `pack` heads of `positions` positions, which lands
+// as rows position * pack + head.
+int encode_q_map(CUtensorMap* map, const void* base, int B, int H, int S, const int64_t* st, int pack, int positions) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B2_LAUNCH_FAILED, "window_fwd: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[4] = {HEAD_DIM, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
+  const cuuint64_t strides[3] = {(cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2, (cuuint64_t)st[0] * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)pack, (cuuint32_t)positions, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_LAUNCH_FAILED, "window_fwd: tensor map encode failed (%d)", (int)r);
+  return B2_OK;
+}
+
 }  // namespace
 
 int64_t window_fwd_workspace_bytes(int B, int H, int Hkv, int Sq, int Sk, int left, int right, int sinks) {
@@ -776,7 +1172,8 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   static PerDeviceSetup per_device;
   const DeviceSlot* slot = nullptr;
   const int setup_status = per_device.get("window_fwd", [](int, DeviceSlot&) -> int {
-    const void* kernels[2] = {(const void*)window_fwd_kernel<false>, (const void*)window_fwd_kernel<true>};
+    const void* kernels[2] = {(const void*)window_tile_kernel, (const void*)window_few_kernel};
+    const int split[2] = {2 * TILE_REGS_SOFTMAX + TILE_REGS_SERVICE, 2 * FEW_REGS_SOFTMAX + FEW_REGS_SERVICE};
     const int bytes[2] = {WinSmem<false>::TOTAL, WinSmem<true>::TOTAL};
     for (int i = 0; i < 2; ++i) {
       const void* f = kernels[i];
@@ -785,20 +1182,23 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
       cudaFuncAttributes fa;
       e = cudaFuncGetAttributes(&fa, f);
       if (e != cudaSuccess) return fail(B2_LAUNCH_FAILED, "window_fwd: attributes: %s", cudaGetErrorString(e));
-      if (2 * B2_FLASH_REGS_SOFTMAX + WIN_REGS_SERVICE > 3 * ((fa.numRegs + 7) / 8 * 8))
-        return fail(B2_LAUNCH_FAILED, "window_fwd: register split %d/%d does not fit %d launch registers",
-                    B2_FLASH_REGS_SOFTMAX, WIN_REGS_SERVICE, fa.numRegs);
+      if (split[i] > 3 * ((fa.numRegs + 7) / 8 * 8))
+        return fail(B2_LAUNCH_FAILED, "window_fwd: a register split of %d does not fit %d launch registers", split[i], fa.numRegs);
     }
     return B2_OK;
   }, &slot);
   if (setup_status != B2_OK) return setup_status;
   const WinPlan plan = make_plan(B, H, Hkv, Sq, Sk, left, right, sinks);
-  CUtensorMap tk, tv;
+  CUtensorMap tq, tk, tv;
   WinArgs a;
   int st = encode_qkv_map(&tk, k, B, Hkv, Sk, ks, &a.k_swap);
   if (st != B2_OK) return st;
   st = encode_qkv_map(&tv, v, B, Hkv, Sk, vs, &a.v_swap);
   if (st != B2_OK) return st;
+  if (!plan.few) {
+    st = encode_q_map(&tq, q, B, H, Sq, qs, plan.pack, plan.tile_pos);
+    if (st != B2_OK) return st;
+  }
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.total_rows = (int64_t)B * Sq * H;
   a.join = plan.join ? 1 : 0;
@@ -814,18 +1214,21 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   a.v_h = vs[1];
   a.v_s = vs[2];
   a.H = H;
-  a.Hkv = Hkv;
   a.share = H / Hkv;
   a.Sq = Sq;
   a.Sk = Sk;
-  a.rows = Sq * a.share;
+  a.pack = plan.pack;
+  a.tile_pos = plan.tile_pos;
+  a.blocks = plan.blocks;
   a.left = left;
   a.right = right;
   a.sinks = left < 0 ? 0 : sinks;
   a.splits = plan.splits;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  const int64_t items = (int64_t)plan.blocks * plan.splits * (H / plan.pack) * B;
+  if (items > 0x7fffffffLL) return fail(B2_TOO_LARGE, "window_fwd: too many work items");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(plan.blocks * plan.splits), (unsigned)Hkv, (unsigned)B);
+  cfg.gridDim = dim3((unsigned)items);
   cfg.blockDim = dim3(NUM_THREADS);
   cfg.dynamicSmemBytes = plan.few ? WinSmem<true>::TOTAL : WinSmem<false>::TOTAL;
   cfg.stream = stream;
@@ -836,8 +1239,8 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = plan.few ? cudaLaunchKernelEx(&cfg, window_fwd_kernel<true>, tk, tv, a)
-                                 : cudaLaunchKernelEx(&cfg, window_fwd_kernel<false>, tk, tv, a);
+  const cudaError_t e = plan.few ? cudaLaunchKernelEx(&cfg, window_few_kernel, tk, tv, a)
+                                 : cudaLaunchKernelEx(&cfg, window_tile_kernel, tq, tk, tv, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(B2_LAUNCH_FAILED, "window_fwd: launch failed: %s", cudaGetErrorString(e));
