@@ -22,15 +22,22 @@ from .ulysses import UlyssesSP
 
 
 def make_block_params(hidden: int = 3072, heads: int = 24, head_dim: int = 128, ffn: int = 8192,
-                      seed: int = 0, device="cuda") -> dict:
+                      seed: int = 0, device="cuda", weights: str = "int8") -> dict:
     """Random-init block: weights ~N(0,0.02) quantised per output channel (symmetric
     int8, scale = absmax/127, round half even, clamp +-127), biases ~N(0,0.01),
-    modulation vectors ~N(0,0.1), norm weights 1 + N(0,0.02)."""
+    modulation vectors ~N(0,0.1), norm weights 1 + N(0,0.02).  `weights="mxfp4"` quantises the
+    same weights (rounded to bf16) to MXFP4 on the device instead: "w4_*" and "s4_*"."""
+    if weights not in ("int8", "mxfp4"):
+        raise ValueError(f"weights must be int8 or mxfp4, got {weights!r}")
     g = torch.Generator(device="cpu").manual_seed(seed)
     p = {}
 
     def qweight(name, n, k):
         w = (torch.randn((n, k), generator=g) * 0.02)
+        if weights == "mxfp4":
+            p["w4_" + name], p["s4_" + name] = ops.quantize_mxfp4(w.to(torch.bfloat16).to(device))
+            p["b_" + name] = (torch.randn((n,), generator=g) * 0.01).to(torch.bfloat16).to(device)
+            return
         scale = (w.abs().amax(-1) / 127.0).clamp(min=1e-30)
         p["wq_" + name] = (w / scale[:, None]).round().clamp(-127, 127).to(torch.int8).to(device)
         p["ws_" + name] = scale.float().to(device)
@@ -72,13 +79,24 @@ def grid_positions(tokens: int, height: int = 22, width: int = 38) -> torch.Tens
 
 
 class DiTBlock:
+    """`window=(left, right)` and `sinks` restrict attention to a sliding window of token positions
+    and the first tokens (`ops.window_fwd_bhsd`; None: full attention).  Parameters with MXFP4
+    weights (`make_block_params(weights="mxfp4")`) run the four linears in that format, on one GPU."""
+
     def __init__(self, params: dict, sp: UlyssesSP | None = None, head_chunks: int = 1,
-                 overlap: bool = True, fuse_residual: bool = True, fuse_swiglu: bool = True):
+                 overlap: bool = True, fuse_residual: bool = True, fuse_swiglu: bool = True,
+                 window: tuple[int, int] | None = None, sinks: int = 0):
         self.p = params
+        self.window, self.sinks = window, sinks
+        if window is None and sinks:
+            raise ValueError("sinks need a window")
+        self.mxfp4 = "w4_qkv" in params
+        if self.mxfp4 and sp is not None and sp.world > 1:
+            raise ValueError("MXFP4 weights run on one GPU: the sequence-parallel ends quantise to int8")
         self.fuse_residual = fuse_residual   # gated residual in the GEMM epilogue where it pays (same bits either way)
         # SwiGLU in fc1's epilogue (same bits either way): the [L, 2*ffn] projection never reaches
         # memory; needs fc1's rows interleaved gate/up in groups of 64, prepared once here
-        self.fuse_swiglu = bool(fuse_swiglu) and params["ffn"] % ops.SWIGLU_GROUP == 0
+        self.fuse_swiglu = bool(fuse_swiglu) and not self.mxfp4 and params["ffn"] % ops.SWIGLU_GROUP == 0
         self._fc1_interleaved = None
         if self.fuse_swiglu:
             self._fc1_interleaved = tuple(ops.interleave_gate_up(params[k]) for k in ("wq_fc1", "ws_fc1", "b_fc1"))
@@ -89,6 +107,8 @@ class DiTBlock:
         self.head_dim = params["head_dim"]
 
     def _attn(self, q, k, v):
+        if self.window is not None:
+            return ops.window_fwd_bhsd(q, k, v, self.head_dim ** -0.5, *self.window, self.sinks)
         return ops.fwd_bhsd(q, k, v, self.head_dim ** -0.5)
 
     def attention(self, qkv: torch.Tensor) -> torch.Tensor:
@@ -121,6 +141,8 @@ class DiTBlock:
         p = self.p
         L = x.shape[0]
         x = x.clone()
+        if self.mxfp4:
+            return self._forward_mxfp4(x, cos, sin, taps)
         q8, s = ops.layernorm_mod_quant(x, p["scale1"], p["shift1"])
         qkv = ops.int8_gemm_dequant(q8, s.view(-1), p["wq_qkv"], p["ws_qkv"], p["b_qkv"])
         qkv = qkv.view(L, 3, self.heads, self.head_dim)
@@ -156,6 +178,21 @@ class DiTBlock:
             q8, s = ops.swiglu_quantize_int8_rowwise(f)
         self._linear_residual(x, p["gate2"], q8, s, p["wq_fc2"], p["ws_fc2"], p["b_fc2"])
         return x
+
+
+    def _forward_mxfp4(self, x, cos, sin, taps):
+        """The same block with MXFP4 linears: every linear quantises its own input, the second FFN
+        projection's with SwiGLU in front."""
+        p = self.p
+        linear = lambda t, name, act=None: ops.mxfp4_linear(t, p["w4_" + name], p["s4_" + name], p["b_" + name], act)  # noqa: E731
+        qkv = linear(ops.layernorm_mod(x, p["scale1"], p["shift1"]), "qkv").view(x.shape[0], 3, self.heads, self.head_dim)
+        ops.qk_norm_rope_(qkv, p["q_norm_w"], p["k_norm_w"], cos, sin)
+        attn_rows = self.attention(qkv)
+        if taps is not None:
+            taps["qkv"], taps["attn"] = qkv, attn_rows
+        ops.gate_residual_(x, linear(attn_rows, "out"), p["gate1"])
+        f = linear(ops.layernorm_mod(x, p["scale2"], p["shift2"]), "fc1")
+        return ops.gate_residual_(x, linear(f, "fc2", "swiglu"), p["gate2"])
 
 
 class GraphedBlock:

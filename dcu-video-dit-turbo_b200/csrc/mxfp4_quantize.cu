@@ -211,6 +211,39 @@ dequantize_int8_rows_kernel(const uint2* __restrict__ q, const float* __restrict
   }
 }
 
+// Widths that are no multiple of 8: q and out start a row at the same place in their vectors, so a warp
+// takes the aligned vectors that a row touches and stores those at its ends element by element.
+__global__ void __launch_bounds__(kThreads)
+dequantize_int8_rows_odd_kernel(const uint2* __restrict__ q, const float* __restrict__ scale, uint4* __restrict__ out,
+                                int64_t M, int K) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); row < M;
+       row += (int64_t)gridDim.x * (kThreads / 32)) {
+    const float s = __ldg(scale + row);
+    const int64_t start = row * K, v0 = start >> 3;
+    const int head = (int)(start & 7), vecs = (head + K + 7) >> 3;
+    for (int c = lane; c < vecs; c += 32) {
+      if (c * 8 >= head && c * 8 + 8 - head <= K) {
+        const uint2 v = __ldg(q + v0 + c);
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = (j < 2 ? v.x : v.y) >> (16 * (j & 1));
+          o[j] = pack_bf16x2_rn((float)(int8_t)(w & 0xff) * s, (float)(int8_t)((w >> 8) & 0xff) * s);
+        }
+        out[v0 + c] = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+        for (int j = 0; j < 8; ++j) {
+          const int col = c * 8 + j - head;
+          if (col < 0 || col >= K) continue;
+          reinterpret_cast<__nv_bfloat16*>(out + v0 + c)[j] =
+              __float2bfloat16_rn((float)reinterpret_cast<const int8_t*>(q + v0 + c)[j] * s);
+        }
+      }
+    }
+  }
+}
+
 // Any width and alignment: one CTA per row, element by element.
 __global__ void __launch_bounds__(kThreads)
 dequantize_int8_rows_generic_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
@@ -288,6 +321,10 @@ int launch_dequantize_int8_rows(const int8_t* q, const float* scale, void* out, 
     const int64_t cap = (int64_t)kNumSMsB200 * 32;
     dequantize_int8_rows_kernel<<<(unsigned)(need < cap ? need : cap), kThreads, 0, stream>>>(
         (const uint2*)q, scale, (uint4*)out, M, kvec);
+  } else if (K <= 0x7ffffff0LL && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && aligned16(out)) {
+    const int64_t need = (M + kThreads / 32 - 1) / (kThreads / 32), cap = (int64_t)kNumSMsB200 * 32;
+    dequantize_int8_rows_odd_kernel<<<(unsigned)(need < cap ? need : cap), kThreads, 0, stream>>>(
+        (const uint2*)q, scale, (uint4*)out, M, (int)K);
   } else {
     const int64_t cap = (int64_t)kNumSMsB200 * 16;
     dequantize_int8_rows_generic_kernel<<<(unsigned)(M < cap ? M : cap), kThreads, 0, stream>>>(

@@ -41,6 +41,19 @@ __device__ __forceinline__ float int8_scale(float absmax, float& inv, bool& zero
 // Round half even of a value within +-127 (a few units in the last place over): low byte of the sum.
 __device__ __forceinline__ uint32_t int8_bits(float v) { return __float_as_uint(v + 12582912.0f) & 0xffu; }
 
+// Asks the vectors v0 .. v0 + vecs of x and residual into L2, one request per 128-byte line.
+template <int TPR, int VPT>
+__device__ __forceinline__ void prefetch_row(const RmsArgs& a, int64_t v0, int vecs, int lane) {
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = lane + i * TPR;
+    if (c < vecs && (lane & 7) == 0) {
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.x + v0 + c));
+      if (a.residual != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.residual + v0 + c));
+    }
+  }
+}
+
 template <int THREADS, int TPR, int VPT, bool MX>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS)
 rmsnorm_residual_kernel(const RmsArgs a) {
@@ -73,16 +86,7 @@ rmsnorm_residual_kernel(const RmsArgs a) {
     // dependent reductions, and what is in flight meanwhile is all that keeps memory busy (int8,
     // 4099 x 5120: 43 -> 31 us, 8192 x 16384: 277 -> 154 us).
     const int64_t next = row + (int64_t)gridDim.x * RPC;
-    if (next < a.M) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = lane + i * TPR;
-        if (c < a.cvec && (lane & 7) == 0) {   // one request per 128-byte line
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.x + next * a.cvec + c));
-          if (a.residual != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.residual + next * a.cvec + c));
-        }
-      }
-    }
+    if (next < a.M) prefetch_row<TPR, VPT>(a, next * a.cvec, a.cvec, lane);
     uint64_t ss2[2] = {0ull, 0ull};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -164,6 +168,122 @@ rmsnorm_residual_kernel(const RmsArgs a) {
   }
 }
 
+// int8 form for widths that are no multiple of 8.  Rows then start anywhere in a 16-byte vector, but x,
+// residual, sum and q all start a row at the same place in theirs, so a row is held as the aligned
+// vectors that it touches: those at its two ends are shared with its neighbours and are stored
+// element by element.  The weight sits differently under every row and is read from shared memory.
+// Bound by instructions (a predicate and a two-byte load per element): 3.1 TB/s at 23638 x 1001 and
+// 2.5 at 8192 x 4099; one CTA per row and two bytes per load reach 1.2 and 2.0.
+template <int THREADS, int TPR, int VPT>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS)
+rmsnorm_residual_quant_odd_kernel(const RmsArgs a, const __nv_bfloat16* __restrict__ weight, int C) {
+  __shared__ float red[2][THREADS / 32];
+  extern __shared__ __nv_bfloat16 w_s[];
+  constexpr int RPC = THREADS / TPR;
+  const int slot = threadIdx.x / TPR;
+  const int lane = threadIdx.x % TPR;
+  for (int c = threadIdx.x; c < C; c += THREADS) w_s[c] = weight[c];
+  __syncthreads();
+  for (int64_t row0 = (int64_t)blockIdx.x * RPC; row0 < a.M; row0 += (int64_t)gridDim.x * RPC) {
+    const int64_t row = row0 + slot;
+    const bool live = row < a.M;
+    const int64_t start = row * C;
+    const int64_t v0 = start >> 3;
+    const int head = (int)(start & 7);                      // elements of the first vector that are not this row's
+    const int vecs = live ? (head + C + 7) >> 3 : 0;
+    // element i of vector v is column v * 8 + i - head
+    uint4 v[VPT], r[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = lane + i * TPR;
+      // the last vector of the last row may reach past the tensor: it is read element by element
+      const bool whole = c < vecs && (c * 8 + 8 - head <= C || row + 1 < a.M);
+      v[i] = whole ? ldg_stream(a.x + v0 + c) : make_uint4(0, 0, 0, 0);
+      r[i] = whole && a.residual != nullptr ? ldg_stream(a.residual + v0 + c) : make_uint4(0, 0, 0, 0);
+      if (c < vecs && !whole) {
+        uint16_t xe[8] = {}, re[8] = {};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c * 8 + j - head < C) {
+            xe[j] = reinterpret_cast<const uint16_t*>(a.x + v0 + c)[j];
+            if (a.residual != nullptr) re[j] = reinterpret_cast<const uint16_t*>(a.residual + v0 + c)[j];
+          }
+        v[i] = make_uint4(xe[0] | xe[1] << 16, xe[2] | xe[3] << 16, xe[4] | xe[5] << 16, xe[6] | xe[7] << 16);
+        r[i] = make_uint4(re[0] | re[1] << 16, re[2] | re[3] << 16, re[4] | re[5] << 16, re[6] | re[7] << 16);
+      }
+    }
+    const int64_t next = row + (int64_t)gridDim.x * RPC;
+    if (next < a.M) prefetch_row<TPR, VPT>(a, (next * C) >> 3, C >> 3, lane);
+    float y[VPT][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = lane + i * TPR;
+      const bool inner = c * 8 >= head && c * 8 + 8 - head <= C;   // all eight elements are this row's
+      uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      if (a.residual != nullptr) {
+        const uint32_t rw[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = bf16x2_add_rn(w[j], rw[j]);
+        if (c < vecs) {
+          if (inner) {
+            a.sum[v0 + c] = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int col = c * 8 + j - head;
+              if (col >= 0 && col < C) reinterpret_cast<uint16_t*>(a.sum + v0 + c)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int col = c * 8 + j - head;
+        const float e = (j & 1) ? bf16hi_to_f32(w[j >> 1]) : bf16lo_to_f32(w[j >> 1]);
+        y[i][j] = c < vecs && col >= 0 && col < C ? e : 0.f;
+        ss = fmaf(y[i][j], y[i][j], ss);
+      }
+    }
+    ss = slot_allreduce<THREADS, TPR>(ss, red[0], slot, SumOp());
+    const float rstd = rsqrtf(ss * a.inv_c + a.eps);
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int col = (lane + i * TPR) * 8 + j - head;
+        const float w = col >= 0 && col < C ? __bfloat162float(w_s[col]) : 0.f;
+        y[i][j] = y[i][j] * rstd * w;
+        most = max(most, __float_as_uint(y[i][j]) & 0x7fffffffu);
+      }
+    const float absmax = slot_allreduce<THREADS, TPR>(__uint_as_float(most), red[1], slot, NanMaxOp());
+    float inv;
+    bool zero_row;
+    const float s = int8_scale(absmax, inv, zero_row);
+    if (!live) continue;
+    if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = s;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = lane + i * TPR;
+      if (c >= vecs) break;
+      uint32_t b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = zero_row ? 0u : int8_bits(y[i][j] * inv);
+      uint2* dst = reinterpret_cast<uint2*>(a.q) + v0 + c;
+      if (c * 8 >= head && c * 8 + 8 - head <= C) {
+        *dst = make_uint2(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24), b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int col = c * 8 + j - head;
+          if (col >= 0 && col < C) reinterpret_cast<uint8_t*>(dst)[j] = (uint8_t)b[j];
+        }
+      }
+    }
+  }
+}
+
 // int8 form for any width and alignment: one CTA per row, which is read three times (the second and
 // third time from L2).
 __global__ void __launch_bounds__(kThreads)
@@ -204,9 +324,10 @@ rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* sum, void* q, void* scale,
                             int64_t M, int64_t C, float eps, bool mx, cudaStream_t stream) {
   const float inv_c = (float)(1.0 / (double)C);
-  const bool vector = C % 8 == 0 && C <= 16384 && aligned16(x) && aligned16(residual) && aligned16(weight) &&
-                      aligned16(sum) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  if (!vector) {
+  const bool aligned = aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(sum) &&
+                       (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  const bool vector = C % 8 == 0 && C <= 16384 && aligned;
+  if (!vector && !(aligned && !mx && C <= 16376)) {
     if (mx) return fail(B2_NOT_WHITELISTED, "rmsnorm_residual_mxfp4: C=%lld exceeds 16384", (long long)C);
     const int64_t cap = (int64_t)kNumSMsB200 * 8;
     rmsnorm_residual_quant_generic_kernel<<<(unsigned)(M < cap ? M : cap), kThreads, 0, stream>>>(
@@ -225,6 +346,26 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
   a.cvec = (int)(C / 8);
   a.inv_c = inv_c;
   a.eps = eps;
+  if (!vector) {
+#define B2_RMS_ODD(THREADS, TPR, VPT)                                                                            \
+  do {                                                                                                           \
+    const int64_t need = (M + THREADS / TPR - 1) / (THREADS / TPR);                                              \
+    const int64_t cap = (int64_t)kNumSMsB200 * 1024 / THREADS;                                                   \
+    rmsnorm_residual_quant_odd_kernel<THREADS, TPR, VPT>                                                         \
+        <<<(unsigned)(need < cap ? need : cap), THREADS, (size_t)C * 2, stream>>>(a, (const __nv_bfloat16*)weight, (int)C); \
+  } while (0)
+    // a row may touch one vector more than its width fills, besides the one that it fills in part
+    const int64_t vecs = (C + 14) / 8;
+    if (vecs <= 32) B2_RMS_ODD(256, 32, 1);
+    else if (vecs <= 64) B2_RMS_ODD(256, 32, 2);
+    else if (vecs <= 128) B2_RMS_ODD(256, 64, 2);
+    else if (vecs <= 256) B2_RMS_ODD(256, 128, 2);
+    else if (vecs <= 512) B2_RMS_ODD(256, 256, 2);
+    else if (vecs <= 1024) B2_RMS_ODD(256, 256, 4);
+    else B2_RMS_ODD(512, 512, 4);
+#undef B2_RMS_ODD
+    return check_launch("rmsnorm_residual_quant");
+  }
   const int64_t rows = mx ? (M + kMxTileRows - 1) / kMxTileRows * kMxTileRows : M;
 #define B2_RMS(THREADS, TPR, VPT)                                                            \
   do {                                                                                       \

@@ -84,7 +84,7 @@ def test_swiglu_quantizer(cuda_pkg, m, k):
     near_border(g * torch.sigmoid(g) * u, R.mx_bytes(s.cpu(), m, k), R.mx_codes(q.cpu()), 1e-5)
 
 
-@pytest.mark.parametrize("m,k", [(1, 8), (5, 3), (77, 1000), (33, 2080), (300, 4096)])
+@pytest.mark.parametrize("m,k", [(1, 8), (5, 3), (77, 1000), (33, 2080), (300, 4096), (1, 1), (100, 7), (65, 1001), (9, 4099)])
 def test_int8_values(cuda_pkg, m, k):
     g = torch.Generator().manual_seed(m + k)
     q = torch.randint(-128, 128, (m, k), dtype=torch.int8, generator=g)

@@ -36,7 +36,9 @@ def check_int8(ops, x, r, w, eps):
 @pytest.mark.parametrize("residual", [True, False])
 @pytest.mark.parametrize("m,c", [(1, 1), (1, 8), (3, 7), (2, 250), (300, 256), (9, 264), (130, 1024), (65, 1032), (33, 2048),
                                  (17, 2056), (70, 3072), (40, 4096), (21, 5120), (19, 8192), (11, 8200), (7, 16384),
-                                 (5, 16392), (3, 20001)])
+                                 (5, 16392), (3, 20001), (200, 7),
+                                 (129, 255), (64, 257), (33, 1001), (40, 1022), (17, 2047), (21, 2051), (9, 4095), (11, 8189),
+                                 (5, 16375), (4, 16379)])
 def test_int8(cuda_pkg, m, c, residual):
     check_int8(cuda_pkg.ops, *inputs(m, c, residual), 1e-6)
 
@@ -107,6 +109,32 @@ def test_many_rows(cuda_pkg):
     assert (s == s[0]).all()
     q, t, _ = ops.rmsnorm_residual_mxfp4(dev(x * scale), dev(r * scale), dev(w), 0.0)
     assert (q == q[0]).all()
+
+
+@pytest.mark.parametrize("c", [1, 5, 63, 1001])
+def test_odd_widths_stay_inside_the_tensors(cuda_pkg, c):
+    """Rows that share vectors with their neighbours, in the middle of larger buffers that stay as
+    they were; and tensors that start anywhere."""
+    m = 37
+    x, r, w = inputs(m, c, True)
+    want = cuda_pkg.ops.rmsnorm_residual_quant(dev(x), dev(r), dev(w))
+    for offset in (0, 8, 3):
+        place = lambda t: torch.cat((torch.full((offset,), 7.0, dtype=t.dtype), t.flatten(), torch.full((9,), 7.0, dtype=t.dtype))).to(DEV)[offset:offset + t.numel()].view(t.shape)  # noqa: E731
+        xo, ro, wo = place(x), place(r), place(w)
+        q, s, total = cuda_pkg.ops.rmsnorm_residual_quant(xo, ro, wo)
+        # another kernel may take over (pointers off a vector's start): the sums run in another order
+        assert torch.equal(total, want[2])
+        assert ((s - want[1]).abs() <= DELTA * want[1]).all() and ((q.int() - want[0].int()).abs() <= 1).all()
+    lib = cuda_pkg._lib.load()
+    stream = torch.cuda.current_stream(DEV).cuda_stream
+    pad = 64
+    total, q = (torch.full((m * c + 2 * pad,), 5, dtype=t, device=DEV) for t in (torch.bfloat16, torch.int8))
+    scale = torch.zeros(m, device=DEV)
+    xd, rd, wd = dev(x), dev(r), dev(w)
+    assert lib.b2_rmsnorm_residual_quant(xd.data_ptr(), rd.data_ptr(), wd.data_ptr(), total.data_ptr() + 2 * pad, q.data_ptr() + pad,
+                                         scale.data_ptr(), m, c, 1e-6, stream) == 0
+    for t, inside in ((total, want[2]), (q, want[0])):
+        assert (t[:pad] == 5).all() and (t[pad + m * c:] == 5).all() and torch.equal(t[pad:pad + m * c].view(m, c), inside)
 
 
 def test_empty_and_refusals(cuda_pkg):
