@@ -130,7 +130,7 @@ struct Span {
   int n;                     // keys of this sequence
   int lo_full, hi_full;      // every row sees every key of [lo_full, hi_full] (and those before `sinks`)
   int steps;                 // this CTA's share of the key tiles
-  int first, sink_steps, win;   // step j is tile first + j while j < sink_steps, win + j from there
+  int first, sink_steps, win;   // step j starts at key first + 128 j while j < sink_steps, at win + 128 j from there
 };
 
 __device__ __forceinline__ int sequence_keys(const int* lengths, int b, int Sk) {
@@ -156,19 +156,23 @@ __device__ __forceinline__ Span make_span(const WinArgs& a, int pos0, int positi
   const int end = last_key(p_max, a.right, s.n) + 1;             // <= 0: nothing is visible
   int total = 0, sink_tiles = 0, win0 = 0;
   if (end > 0) {
-    win0 = first_key(p_min, a.left) / BLOCK_N;
-    sink_tiles = min((min(a.sinks, end) + BLOCK_N - 1) / BLOCK_N, win0);
-    total = sink_tiles + max((end + BLOCK_N - 1) / BLOCK_N - win0, 0);
+    // Tiles of the window start at its first key, not at a multiple of 128 (which would take two
+    // thirds of a tile more on average), behind the tiles of the first keys where those reach into it.
+    const int begin = first_key(p_min, a.left);
+    sink_tiles = (min(min(a.sinks, begin), end) + BLOCK_N - 1) / BLOCK_N;
+    win0 = max(begin, sink_tiles * BLOCK_N);
+    total = sink_tiles + max(end - win0 + BLOCK_N - 1, 0) / BLOCK_N;
   }
-  s.first = (int)((int64_t)total * split / a.splits);
-  s.steps = (int)((int64_t)total * (split + 1) / a.splits) - s.first;
-  s.sink_steps = sink_tiles - s.first;
-  s.win = win0 - sink_tiles + s.first;
+  const int step0 = (int)((int64_t)total * split / a.splits);
+  s.steps = (int)((int64_t)total * (split + 1) / a.splits) - step0;
+  s.first = step0 * BLOCK_N;
+  s.sink_steps = sink_tiles - step0;
+  s.win = win0 + (step0 - sink_tiles) * BLOCK_N;
   return s;
 }
 // first key of the CTA's step j
 __device__ __forceinline__ int step_key(const Span& s, int j) {
-  return ((j < s.sink_steps ? s.first : s.win) + j) * BLOCK_N;
+  return (j < s.sink_steps ? s.first : s.win) + j * BLOCK_N;
 }
 // some row of the CTA does not see the whole tile
 __device__ __forceinline__ bool is_mixed(const WinArgs& a, const Span& s, int key0) {
