@@ -85,7 +85,7 @@ _timer: LaunchTimer | None = None
 
 def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> None:
     global launch_count
-    lib = _lib.load()
+    fn = getattr(_lib.load(), name)
     timer = _timer
     if timer is not None:
         stream = torch.cuda.current_stream(t.device)
@@ -93,10 +93,11 @@ def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> No
         e0.record(stream)
     if t.get_device() != torch.cuda.current_device():
         with torch.cuda.device(t.device):
-            st = getattr(lib, name)(*args)
+            st = fn(*args)
     else:
-        st = getattr(lib, name)(*args)
-    _lib.check(st, name)
+        st = fn(*args)
+    if st:
+        _lib.check(st, name)
     if timer is not None:
         e1.record(stream)
         timer._records.append((name, e0, e1, work))
@@ -106,11 +107,14 @@ def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> No
 def _require_vector(v: torch.Tensor, like: torch.Tensor, numel: int, dtype, what: str) -> None:
     """A per-column operand handed to the C ABI as a raw pointer: right dtype, on the same
     CUDA device as the data, contiguous, with exactly `numel` elements."""
-    _require(torch.is_tensor(v) and v.is_cuda and v.device == like.device,
-             f"{what} must be on the same CUDA device as the data")
-    _require(v.dtype == dtype, f"{what} must be {str(dtype).replace('torch.', '')}")
-    _require(v.is_contiguous(), f"{what} must be contiguous")
-    _require(v.numel() == numel, f"{what} must contain exactly {numel} values")
+    if not (torch.is_tensor(v) and v.is_cuda and v.get_device() == like.get_device()):
+        raise RuntimeError(f"{what} must be on the same CUDA device as the data")
+    if v.dtype != dtype:
+        raise RuntimeError(f"{what} must be {str(dtype).replace('torch.', '')}")
+    if not v.is_contiguous():
+        raise RuntimeError(f"{what} must be contiguous")
+    if v.numel() != numel:
+        raise RuntimeError(f"{what} must contain exactly {numel} values")
 
 
 def quantize_int8_rowwise(x: torch.Tensor):
@@ -666,7 +670,7 @@ def dequantize_int8_rowwise(q: torch.Tensor, scale: torch.Tensor) -> torch.Tenso
              "q must be a contiguous CUDA int8 [M,K] tensor")
     _require_vector(scale, q, q.shape[0], torch.float32, "scale")
     m, k = q.shape
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=q.device)
+    out = torch.empty_like(q, dtype=torch.bfloat16)
     if m and k:
         _call("b2_dequantize_int8_rowwise", q, q.data_ptr(), scale.data_ptr(), out.data_ptr(), m, k, _stream(q),
               work=("hbm", 3 * m * k + 4 * m))
@@ -722,15 +726,17 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
 # ---- RMSNorm with the residual's addition (no counterpart in the reference) ---------
 
 def _rmsnorm_inputs(x, residual, weight, eps):
-    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.shape[1] > 0,
-             "x must be a contiguous CUDA bf16 [M,C] tensor")
+    """Checks the norm's inputs; returns the tensor for the sum (x itself without a residual)."""
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.shape[1] > 0):
+        raise RuntimeError("x must be a contiguous CUDA bf16 [M,C] tensor")
     _require_vector(weight, x, x.shape[1], torch.bfloat16, "weight")
-    _require(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative")
+    if not (eps >= 0.0 and eps != math.inf):
+        raise RuntimeError("eps must be finite and not negative")
     if residual is None:
         return x
-    _require(residual.is_cuda and residual.device == x.device and residual.dtype == torch.bfloat16
-             and residual.shape == x.shape and residual.is_contiguous(),
-             "residual must be a contiguous bf16 tensor of x's shape on the same device")
+    if not (residual.dtype == torch.bfloat16 and residual.get_device() == x.get_device() and residual.shape == x.shape
+            and residual.is_contiguous()):
+        raise RuntimeError("residual must be a contiguous bf16 tensor of x's shape on the same device")
     return torch.empty_like(x)
 
 
@@ -741,11 +747,11 @@ def rmsnorm_residual_quant(x: torch.Tensor, residual: torch.Tensor | None, weigh
     is x itself."""
     total = _rmsnorm_inputs(x, residual, weight, eps)
     m, c = x.shape
-    q = torch.empty((m, c), dtype=torch.int8, device=x.device)
+    q = torch.empty_like(x, dtype=torch.int8)
     s = torch.empty((m, 1), dtype=torch.float32, device=x.device)
     if m:
-        _call("b2_rmsnorm_residual_quant", x, x.data_ptr(), _ptr(residual), weight.data_ptr(),
-              None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+        _call("b2_rmsnorm_residual_quant", x, x.data_ptr(), None if residual is None else residual.data_ptr(),
+              weight.data_ptr(), None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
               work=("hbm", (3 if residual is None else 7) * m * c + 4 * m))
     return [q, s, total]
 
@@ -758,8 +764,8 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
     _require(c % MX_BLOCK == 0 and c <= 16384, "the width must be a multiple of 32, at most 16384")
     q, s = _mx_empty(m, c, x.device)
     if m:
-        _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), _ptr(residual), weight.data_ptr(),
-              None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+        _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), None if residual is None else residual.data_ptr(),
+              weight.data_ptr(), None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
               work=("hbm", (2 if residual is None else 6) * m * c + m * c // 2 + m * c // MX_BLOCK))
     return [q, s, total]
 

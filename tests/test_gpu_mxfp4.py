@@ -101,7 +101,7 @@ def product_bound(a, w, want):
 
 @pytest.mark.parametrize("m,n,k", [(1, 8, 32), (1, 264, 4096), (3, 16, 64), (16, 520, 96), (31, 1000, 256), (64, 256, 544),
                                    (65, 128, 512), (128, 256, 256), (129, 264, 288), (200, 384, 2080), (256, 512, 1024),
-                                   (257, 648, 416), (1000, 1000, 1056), (2049, 2312, 4128)])
+                                   (257, 648, 416), (1000, 1000, 1056), (2049, 2312, 4128), (65, 19464, 96)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_product(cuda_pkg, m, n, k, bias):
     a, sa, av = (t.to(DEV) for t in R.random_mx(m, k, m + k))
