@@ -682,8 +682,10 @@ int launch_mxfp4_gemm(const uint8_t* A, const uint8_t* a_scale, const uint8_t* W
   // one 128 x 128 tile (or a share of its K) per SM, while there are SMs
   const int64_t small_tiles = ((M + BM - 1) / BM) * ((N + SBN - 1) / SBN);
   if (small_tiles <= slot->a) {
+    // clusters of four and eight leave SMs without a place (132 and 120 of 148 can be used)
     int splits = 1;
-    while (splits < 8 && small_tiles * splits * 2 <= slot->a && splits * 2 <= a.k_blocks) splits *= 2;
+    for (int s = 2; s <= 8 && s <= a.k_blocks; s *= 2)
+      if (small_tiles * s <= (s == 2 ? slot->a : s == 4 ? 132 : 120)) splits = s;
     int st = encode_operand(&ta, A, M, K, BM);
     if (st == B2_OK) st = encode_operand(&tb, W, N, K, SBN);
     if (st == B2_OK) st = encode_scales(&tsa, a_scale, M, K, 1);

@@ -196,8 +196,8 @@ rmsnorm_residual_quant_odd_kernel(const RmsArgs a, const __nv_bfloat16* __restri
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = lane + i * TPR;
-      // the last vector of the last row may reach past the tensor: it is read element by element
-      const bool whole = c < vecs && (c * 8 + 8 - head <= C || row + 1 < a.M);
+      // the tensor's last vector may be a part of one: it is read element by element
+      const bool whole = c < vecs && (v0 + c) * 8 + 8 <= a.M * C;
       v[i] = whole ? ldg_stream(a.x + v0 + c) : make_uint4(0, 0, 0, 0);
       r[i] = whole && a.residual != nullptr ? ldg_stream(a.residual + v0 + c) : make_uint4(0, 0, 0, 0);
       if (c < vecs && !whole) {

@@ -53,7 +53,7 @@ class LaunchTimer:
             block.forward(x, cos, sin)
         for rec in timer.results(): ...   # {"name", "ms", "bound", "work"}
 
-    `bound` names the roofline that limits the kernel ("hbm", "int8" or "bf16") and `work`
+    `bound` names the roofline that limits the kernel ("hbm", "int8", "bf16", "mxfp4" or "nvlink") and `work`
     its algorithmic bytes (hbm) or operations per launch, so a caller can turn `ms` into
     GB/s or TOP/s.  Events are recorded on PyTorch's current stream of the tensor's device
     (the stream the kernel is enqueued on); nothing synchronises until `results()`."""
