@@ -117,12 +117,14 @@ __device__ __forceinline__ uint32_t exp_pair(uint32_t sa, uint32_t sb, uint64_t 
   return pack_bf16x2_rn(e0, e1);
 }
 
-// 16 scores of one thread (one chunk) -> 8 packed bf16 probabilities.
+// 16 scores of one thread (one chunk) -> 8 packed bf16 probabilities; EMU_MASK: the pairs whose
+// exponential runs on the FMA pipe.
+template <int EMU_MASK = B2_FLASH_EMU_MASK>
 __device__ __forceinline__ void exp_chunk(const uint32_t* s, uint32_t (&p)[8], uint64_t sl2x2,
                                           uint64_t nmsx2, uint64_t (&sm2)[4]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if ((B2_FLASH_EMU_MASK >> i) & 1)
+    if ((EMU_MASK >> i) & 1)
       p[i] = exp_pair<true>(s[2 * i], s[2 * i + 1], sl2x2, nmsx2, sm2[i & 3]);
     else
       p[i] = exp_pair<false>(s[2 * i], s[2 * i + 1], sl2x2, nmsx2, sm2[i & 3]);

@@ -300,6 +300,12 @@ struct Row {
       : key_first(first_key(position, a.left)), key_last(last_key(position, a.right, n)), live(exists) {}
 };
 
+// One of eight score pairs takes its exponential on the FMA pipe (two in flash_fwd.cu): with masks and
+// work items around the steps the softmax warps are short of issue slots before the exp2 unit is full.
+// One against two: 0.7 to 2.8 % less time over windows from 511 to whole sequences; none loses 2 % on
+// the long ones, three 6 %.
+constexpr int WIN_EMU_MASK = 0x02;
+
 // One step of one tile: scores from tensor memory -> masked -> P in their place, O rescaled if the
 // maximum grew (`rescale` is false on the row's first step, when O holds nothing).  `publish(part)`
 // hands a half of P to the MMA issuer.
@@ -356,7 +362,7 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     uint32_t p[8];
-    exp_chunk(&s[16 * q], p, sl2x2, nmsx2, sm2);
+    exp_chunk<WIN_EMU_MASK>(&s[16 * q], p, sl2x2, nmsx2, sm2);
     tmem_st_32x32b_x8(s_tmem + 8 * q, p);   // P takes the first half of S
     if ((q + 1) % 4 == 0) {
       tmem_wait_st();
