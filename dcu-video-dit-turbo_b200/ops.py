@@ -85,7 +85,7 @@ _timer: LaunchTimer | None = None
 
 def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> None:
     global launch_count
-    fn = getattr(_lib.load(), name)
+    fn = getattr(_lib.current(), name)
     timer = _timer
     if timer is not None:
         stream = torch.cuda.current_stream(t.device)
@@ -595,6 +595,11 @@ def gate_residual_(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor) -> torc
 # ---- MXFP4 (no counterpart in the reference) -------------------------------------
 
 MX_BLOCK = 32    # columns that share a scale
+_BF16, _F32, _I8, _U8 = torch.bfloat16, torch.float32, torch.int8, torch.uint8
+
+# These operators are called for single tokens, where the host's time is the call's: conditions are
+# tested together and told apart only when one fails, and tensors are made from positional sizes
+# (0.7 us less each than from a tuple).
 
 
 def mxfp4_scale_shape(rows: int, columns: int) -> tuple[int, int, int]:
@@ -603,38 +608,42 @@ def mxfp4_scale_shape(rows: int, columns: int) -> tuple[int, int, int]:
     return (-(-rows // 128), -(-columns // 128), 512)
 
 
-def _mx_empty(rows: int, columns: int, device):
-    return (torch.empty((rows, columns // 2), dtype=torch.uint8, device=device),
-            torch.empty(mxfp4_scale_shape(rows, columns), dtype=torch.uint8, device=device))
-
-
 def _require_mx(q: torch.Tensor, s: torch.Tensor, what: str) -> tuple[int, int]:
     """Checks a quantised matrix (elements, scales); returns its rows and columns."""
-    if not (q.is_cuda and s.is_cuda and q.get_device() == s.get_device()):
-        raise RuntimeError(f"{what} and its scales must be on the same CUDA device")
-    if q.dtype != torch.uint8 or s.dtype != torch.uint8:
-        raise RuntimeError(f"{what} and its scales must be uint8")
-    if q.dim() != 2 or not q.is_contiguous() or not s.is_contiguous():
-        raise RuntimeError(f"{what} must be a contiguous [M, K/2] tensor with contiguous scales")
-    m, k = q.shape
-    k *= 2
-    if k % MX_BLOCK:
-        raise RuntimeError(f"{what} must have a multiple of {MX_BLOCK} columns")
-    if s.shape != mxfp4_scale_shape(m, k):
-        raise RuntimeError(f"the scales of {what} must have shape {mxfp4_scale_shape(m, k)}, got {tuple(s.shape)}")
-    return m, k
+    if q.dim() == 2 and s.dim() == 3:
+        m, k = q.shape
+        k *= 2
+        if (q.dtype == s.dtype == _U8 and q.is_cuda and q.get_device() == s.get_device() and q.is_contiguous()
+                and s.is_contiguous() and k % MX_BLOCK == 0 and s.shape == (-(-m // 128), -(-k // 128), 512)):
+            return m, k
+    _require(q.is_cuda and s.is_cuda and q.device == s.device, f"{what} and its scales must be on the same CUDA device")
+    _require(q.dtype == _U8 and s.dtype == _U8, f"{what} and its scales must be uint8")
+    _require(q.dim() == 2 and q.is_contiguous() and s.is_contiguous(),
+             f"{what} must be a contiguous [M, K/2] tensor with contiguous scales")
+    m, k = q.shape[0], 2 * q.shape[1]
+    _require(k % MX_BLOCK == 0, f"{what} must have a multiple of {MX_BLOCK} columns")
+    raise RuntimeError(f"the scales of {what} must have shape {mxfp4_scale_shape(m, k)}, got {tuple(s.shape)}")
+
+
+def _require_rows(x: torch.Tensor) -> None:
+    """Checks a quantiser's input."""
+    if x.dtype == _BF16 and x.is_cuda and x.dim() == 2 and x.is_contiguous():
+        return
+    _require(x.is_cuda, "input must be on the CUDA device")
+    _require(x.is_contiguous(), "input must be contiguous")
+    _require(x.dtype == _BF16, "input must be bfloat16")
+    raise RuntimeError("input must be a two-dimensional tensor")
 
 
 def _quantize_mxfp4(name: str, x: torch.Tensor, halves: int):
-    _require(x.is_cuda, "input must be on the CUDA device")
-    _require(x.is_contiguous(), "input must be contiguous")
-    _require(x.dtype == torch.bfloat16, "input must be bfloat16")
-    _require(x.dim() == 2, "input must be a two-dimensional tensor")
+    _require_rows(x)
     m, width = x.shape
-    k = width // halves
     if width % (halves * MX_BLOCK):
         raise RuntimeError(f"input width must be a multiple of {halves * MX_BLOCK}")
-    q, s = _mx_empty(m, k, x.device)
+    k = width // halves
+    device = x.device
+    q = torch.empty(m, k // 2, dtype=_U8, device=device)
+    s = torch.empty(-(-m // 128), -(-k // 128), 512, dtype=_U8, device=device)
     if m and k:
         _call(name, x, x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, _stream(x),
               work=("hbm", 2 * halves * m * k + m * k // 2 + m * k // MX_BLOCK))
@@ -645,7 +654,8 @@ def quantize_mxfp4(x: torch.Tensor):
     """bf16 [M,K] -> [uint8 [M,K/2], uint8 scales]: microscaled 4-bit floating point, a power-of-two
     scale 2^(floor(log2(max|x|)) - 2) per 32 columns, elements +-{0, .5, 1, 1.5, 2, 3, 4, 6} to the
     nearest with ties to the even code, two per byte (even column in the low half).  The scales'
-    layout is `mxfp4_scale_shape`'s, the one `mxfp4_gemm` reads."""
+    layout is `mxfp4_scale_shape`'s, the one `mxfp4_gemm` reads.  A block with a NaN or an infinity
+    gets the NaN scale 255 and zero elements."""
     return _quantize_mxfp4("b2_quantize_mxfp4", x, 1)
 
 
@@ -657,7 +667,7 @@ def swiglu_quantize_mxfp4(x: torch.Tensor):
 def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
     """bf16 [M,K]: the values of a quantised matrix."""
     m, k = _require_mx(q, s, "the matrix")
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=q.device)
+    out = torch.empty(m, k, dtype=_BF16, device=q.device)
     if m and k:
         _call("b2_dequantize_mxfp4", q, q.data_ptr(), s.data_ptr(), out.data_ptr(), m, k, _stream(q),
               work=("hbm", 2 * m * k + m * k // 2 + m * k // MX_BLOCK))
@@ -666,15 +676,24 @@ def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
 
 def dequantize_int8_rowwise(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """bf16 [M,K] = q * scale[row]: the values of rowwise int8 (scale fp32, M values)."""
-    _require(q.is_cuda and q.dtype == torch.int8 and q.dim() == 2 and q.is_contiguous(),
-             "q must be a contiguous CUDA int8 [M,K] tensor")
-    _require_vector(scale, q, q.shape[0], torch.float32, "scale")
+    if not (q.dtype == _I8 and q.is_cuda and q.dim() == 2 and q.is_contiguous()):
+        raise RuntimeError("q must be a contiguous CUDA int8 [M,K] tensor")
     m, k = q.shape
-    out = torch.empty_like(q, dtype=torch.bfloat16)
+    _require_vector(scale, q, m, _F32, "scale")
+    out = torch.empty_like(q, dtype=_BF16)
     if m and k:
         _call("b2_dequantize_int8_rowwise", q, q.data_ptr(), scale.data_ptr(), out.data_ptr(), m, k, _stream(q),
               work=("hbm", 3 * m * k + 4 * m))
     return out
+
+
+def _mx_product_shape(device, n: int, k: int, bias) -> int:
+    """Checks an MXFP4 product's width, depth and bias; returns the bias kind."""
+    if n % 8:
+        raise RuntimeError("the output width must be a multiple of 8")
+    if k <= 0:
+        raise RuntimeError("the inner dimension must be positive")
+    return BIAS_NONE if bias is None else _bias_kind(bias, n, device)
 
 
 def mxfp4_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -684,15 +703,16 @@ def mxfp4_gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     rounding.  N must be a multiple of 8."""
     m, k = _require_mx(a, a_scale, "a")
     n, kw = _require_mx(w, w_scale, "w")
-    _require(w.device == a.device, "all inputs must be on the same device")
-    _require(k == kw, "shape mismatch")
-    _require(n % 8 == 0, "the output width must be a multiple of 8")
-    _require(k > 0, "the inner dimension must be positive")
-    kind = _bias_kind(bias, n, a.device)
-    out = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+    device = a.device
+    if w.get_device() != a.get_device():
+        raise RuntimeError("all inputs must be on the same device")
+    if k != kw:
+        raise RuntimeError("shape mismatch")
+    kind = _mx_product_shape(device, n, k, bias)
+    out = torch.empty(m, n, dtype=_BF16, device=device)
     if m and n:
         _call("b2_mxfp4_gemm", a, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-              _ptr(bias) if kind else None, kind, out.data_ptr(), m, n, k, _stream(a), work=("mxfp4", 2 * m * n * k))
+              bias.data_ptr() if kind else None, kind, out.data_ptr(), m, n, k, _stream(a), work=("mxfp4", 2 * m * n * k))
     return out
 
 
@@ -700,24 +720,24 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
                  input_act: str | None = None) -> torch.Tensor:
     """One C call for (activation) -> quantize -> product.  x bf16 [M,K] (or [M,2K] with
     input_act="swiglu"); w, w_scale a quantised [N,K] weight."""
-    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous(),
-             "x must be a contiguous CUDA bf16 [M,K] tensor")
+    if not (x.dtype == _BF16 and x.is_cuda and x.dim() == 2 and x.is_contiguous()):
+        raise RuntimeError("x must be a contiguous CUDA bf16 [M,K] tensor")
     n, k = _require_mx(w, w_scale, "w")
     act = {None: ACT_NONE, "swiglu": ACT_SWIGLU}.get(input_act, -1)
     if act < 0:
         raise RuntimeError(f"unknown input activation {input_act!r}")
-    _require(w.device == x.device, "all inputs must be on the same device")
-    width = 2 * k if act == ACT_SWIGLU else k
-    if x.shape[1] != width:
-        raise ValueError(f"Input and weight inner dimensions must match, got {x.shape[1]} and {width}")
-    _require(n % 8 == 0, "the output width must be a multiple of 8")
-    _require(k > 0, "the inner dimension must be positive")
-    m = x.shape[0]
-    kind = _bias_kind(bias, n, x.device)
-    out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    if w.get_device() != x.get_device():
+        raise RuntimeError("all inputs must be on the same device")
+    m, width = x.shape
+    if width != (2 * k if act == ACT_SWIGLU else k):
+        raise ValueError(f"Input and weight inner dimensions must match, got {width} and {2 * k if act else k}")
+    device = x.device
+    kind = _mx_product_shape(device, n, k, bias)
+    out = torch.empty(m, n, dtype=_BF16, device=device)
     if m and n:
-        qs, ss = _mx_empty(m, k, x.device)
-        _call("b2_mxfp4_linear", x, x.data_ptr(), act, w.data_ptr(), w_scale.data_ptr(), _ptr(bias) if kind else None,
+        qs = torch.empty(m, k // 2, dtype=_U8, device=device)
+        ss = torch.empty(-(-m // 128), -(-k // 128), 512, dtype=_U8, device=device)
+        _call("b2_mxfp4_linear", x, x.data_ptr(), act, w.data_ptr(), w_scale.data_ptr(), bias.data_ptr() if kind else None,
               kind, out.data_ptr(), qs.data_ptr(), ss.data_ptr(), m, n, k, _stream(x), launches=2,
               work=("mxfp4", 2 * m * n * k))
     return out
@@ -727,14 +747,14 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: 
 
 def _rmsnorm_inputs(x, residual, weight, eps):
     """Checks the norm's inputs; returns the tensor for the sum (x itself without a residual)."""
-    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.shape[1] > 0):
+    if not (x.dtype == _BF16 and x.is_cuda and x.dim() == 2 and x.is_contiguous() and x.shape[1] > 0):
         raise RuntimeError("x must be a contiguous CUDA bf16 [M,C] tensor")
-    _require_vector(weight, x, x.shape[1], torch.bfloat16, "weight")
+    _require_vector(weight, x, x.shape[1], _BF16, "weight")
     if not (eps >= 0.0 and eps != math.inf):
         raise RuntimeError("eps must be finite and not negative")
     if residual is None:
         return x
-    if not (residual.dtype == torch.bfloat16 and residual.get_device() == x.get_device() and residual.shape == x.shape
+    if not (residual.dtype == _BF16 and residual.get_device() == x.get_device() and residual.shape == x.shape
             and residual.is_contiguous()):
         raise RuntimeError("residual must be a contiguous bf16 tensor of x's shape on the same device")
     return torch.empty_like(x)
@@ -744,15 +764,16 @@ def rmsnorm_residual_quant(x: torch.Tensor, residual: torch.Tensor | None, weigh
     """sum = bf16(x + residual), y = sum / sqrt(mean(sum^2) + eps) * weight in fp32, quantised to
     int8 rows in the same pass: [q int8 [M,C], scale fp32 [M,1], sum bf16 [M,C]] with
     scale = max(max|y| / 127, 1e-30) and q = round half even(y / scale).  Without a residual, sum
-    is x itself."""
+    is x itself.  A row with a NaN or an infinity keeps it in its scale and has zero elements."""
     total = _rmsnorm_inputs(x, residual, weight, eps)
     m, c = x.shape
-    q = torch.empty_like(x, dtype=torch.int8)
-    s = torch.empty((m, 1), dtype=torch.float32, device=x.device)
+    q = torch.empty_like(x, dtype=_I8)
+    s = torch.empty(m, 1, dtype=_F32, device=x.device)
     if m:
-        _call("b2_rmsnorm_residual_quant", x, x.data_ptr(), None if residual is None else residual.data_ptr(),
-              weight.data_ptr(), None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
-              work=("hbm", (3 if residual is None else 7) * m * c + 4 * m))
+        add = residual is not None
+        _call("b2_rmsnorm_residual_quant", x, x.data_ptr(), residual.data_ptr() if add else None, weight.data_ptr(),
+              total.data_ptr() if add else None, q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+              work=("hbm", (7 if add else 3) * m * c + 4 * m))
     return [q, s, total]
 
 
@@ -761,12 +782,16 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
     C must be a multiple of 32, at most 16384."""
     total = _rmsnorm_inputs(x, residual, weight, eps)
     m, c = x.shape
-    _require(c % MX_BLOCK == 0 and c <= 16384, "the width must be a multiple of 32, at most 16384")
-    q, s = _mx_empty(m, c, x.device)
+    if c % MX_BLOCK or c > 16384:
+        raise RuntimeError("the width must be a multiple of 32, at most 16384")
+    device = x.device
+    q = torch.empty(m, c // 2, dtype=_U8, device=device)
+    s = torch.empty(-(-m // 128), -(-c // 128), 512, dtype=_U8, device=device)
     if m:
-        _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), None if residual is None else residual.data_ptr(),
-              weight.data_ptr(), None if residual is None else total.data_ptr(), q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
-              work=("hbm", (2 if residual is None else 6) * m * c + m * c // 2 + m * c // MX_BLOCK))
+        add = residual is not None
+        _call("b2_rmsnorm_residual_mxfp4", x, x.data_ptr(), residual.data_ptr() if add else None, weight.data_ptr(),
+              total.data_ptr() if add else None, q.data_ptr(), s.data_ptr(), m, c, eps, _stream(x),
+              work=("hbm", (6 if add else 2) * m * c + m * c // 2 + m * c // MX_BLOCK))
     return [q, s, total]
 
 
@@ -789,37 +814,44 @@ def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     and (j >= p - left or j < sinks); -1 lifts the limit of a side (right=0: causal).  A query that
     sees no key gives zeros, and what lies in keys or values that a query does not see has no effect
     on it.  Returns the [B,H,Sq,128] transpose view of a fresh contiguous [B,Sq,H,128] tensor."""
-    _require(q.is_cuda and k.is_cuda and v.is_cuda, "q, k, and v must be on a CUDA device")
-    _require(q.dtype == torch.bfloat16, "kernel requires BF16 q")
-    _require(k.dtype == v.dtype == torch.bfloat16, "q, k, and v must have the same dtype")
-    _require(q.get_device() == k.get_device() == v.get_device(), "q, k, and v must be on the same CUDA device")
-    _require(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, and v must use BHSD layout")
+    if not (q.dtype == k.dtype == v.dtype == _BF16 and q.is_cuda and q.get_device() == k.get_device() == v.get_device()
+            and q.dim() == k.dim() == v.dim() == 4):
+        _require(q.is_cuda and k.is_cuda and v.is_cuda, "q, k, and v must be on a CUDA device")
+        _require(q.dtype == _BF16, "kernel requires BF16 q")
+        _require(k.dtype == v.dtype == _BF16, "q, k, and v must have the same dtype")
+        _require(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, and v must use BHSD layout")
+        raise RuntimeError("q, k, and v must be on the same CUDA device")
     b, h, sq, d = q.shape
     _, hkv, sk, _ = k.shape
-    _require(k.shape == v.shape == (b, hkv, sk, d), "k and v must have the same shape and q's batch and head dimension")
-    _require(d == 128, "kernel requires head dimension 128")
-    _require(b > 0 and h > 0 and sq > 0 and hkv > 0 and sk > 0, "batch, heads, and sequence lengths must be positive")
-    _require(h % hkv == 0, "the query heads must be a multiple of the key heads")
     qb, qh, qs, qd = q.stride()
     kb, kh, ks, kd = k.stride()
     vb, vh, vs, vd = v.stride()
-    _require(qd == 1 and kd == 1 and vd == 1, "q, k, and v must have contiguous last dimensions")
     scale = float(softmax_scale)
-    _require(math.isfinite(scale) and scale > 0.0, "softmax_scale must be finite and positive")
     left, right, sinks = int(left), int(right), int(sinks)
-    _require(left >= -1 and right >= -1 and sinks >= 0, "left and right must be at least -1, sinks at least 0")
+    if not (k.shape == v.shape == (b, hkv, sk, d) and d == 128 and b and h and sq and hkv and sk and h % hkv == 0
+            and qd == kd == vd == 1 and 0.0 < scale < math.inf and left >= -1 and right >= -1 and sinks >= 0):
+        _require(k.shape == v.shape == (b, hkv, sk, d), "k and v must have the same shape and q's batch and head dimension")
+        _require(d == 128, "kernel requires head dimension 128")
+        _require(b > 0 and h > 0 and sq > 0 and hkv > 0 and sk > 0, "batch, heads, and sequence lengths must be positive")
+        _require(h % hkv == 0, "the query heads must be a multiple of the key heads")
+        _require(qd == 1 and kd == 1 and vd == 1, "q, k, and v must have contiguous last dimensions")
+        _require(math.isfinite(scale) and scale > 0.0, "softmax_scale must be finite and positive")
+        raise RuntimeError("left and right must be at least -1, sinks at least 0")
     # nothing lies further away than the sequences are long
-    left, right, sinks = min(left, sk + sq), min(right, sk + sq), min(sinks, sk)
+    far = sk + sq
+    left, right, sinks = min(left, far), min(right, far), min(sinks, sk)
+    lengths = None
     if kv_lengths is not None:
         _require_vector(kv_lengths, q, b, torch.int32, "kv_lengths")
-    storage = torch.empty((b, sq, h, d), dtype=torch.bfloat16, device=q.device)
+        lengths = kv_lengths.data_ptr()
+    device = q.device
+    storage = torch.empty(b, sq, h, d, dtype=_BF16, device=device)
     need = _window_workspace(b, h, hkv, sq, sk, left, right, sinks)
-    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    workspace = torch.empty(need, dtype=_U8, device=device) if need else None
     span = sk if left < 0 or right < 0 else min(sk, left + right + 1)
     _call("b2_window_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), storage.data_ptr(),
-          workspace.data_ptr() if need else None, need, None if kv_lengths is None else kv_lengths.data_ptr(), b, h, hkv,
-          sq, sk, qb, qh, qs, kb, kh, ks, vb, vh, vs, scale, left, right, sinks, _stream(q),
-          launches=2 if need else 1, work=("bf16", 4 * b * h * sq * span * d))
+          workspace.data_ptr() if need else None, need, lengths, b, h, hkv, sq, sk, qb, qh, qs, kb, kh, ks, vb, vh, vs,
+          scale, left, right, sinks, _stream(q), launches=2 if need else 1, work=("bf16", 4 * b * h * sq * span * d))
     return storage.transpose(1, 2)
 
 
