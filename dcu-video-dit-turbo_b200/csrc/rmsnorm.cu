@@ -8,6 +8,7 @@
 // Bound by memory: 4 bytes in and 2 + 1 (2 + 17/32) bytes out per element.  A row is held by TPR
 // threads in registers from its only read to its quantised write; y is never rounded to bf16 in
 // between.  A thread keeps the same columns of every row, so the weight is read once per CTA.
+// Measured: int8 109099 x 3072 369 us = 6.36 TB/s, 23638 x 3072 86 us = 5.9; MXFP4 356 and 84 us.
 // The int8 scale divides by the fp32 scale that is stored, so q * scale is within half a step of y.
 #include "b2_common.cuh"
 #include "b2_launch.h"
