@@ -384,20 +384,27 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
 }
 static_assert(P_PARTS == 2, "P is published in halves");
 
-// Adds the non-finite values that the fix warps took out of the mixed tiles to 32 columns of a row that
-// sees them: the steps first, first + stride, ... of the item.
+// Adds the non-finite values that the fix warps took out of the mixed tiles to a stored row (in fp32, or in
+// bf16 where it is final: an infinity or a NaN is the same there) that sees them: the steps first,
+// first + stride, ... of the item.
 __device__ __forceinline__ void add_nonfinite(const WinArgs& a, const Span& span, const Row& row, int first, int stride,
-                                              int steps, int hkv, int b, int c, uint32_t (&o)[32]) {
+                                              int steps, int hkv, int b, float* part, __nv_bfloat16* out) {
+#pragma unroll 1
   for (int u = first; u < steps; u += stride) {
     const int key0 = step_key(span, u);
     if (!is_mixed(a, span, key0)) continue;
+#pragma unroll 1
     for (int j = key0; j < key0 + BLOCK_N && j <= row.key_last; ++j) {
       if (j < row.key_first && j >= a.sinks) continue;
-      const __nv_bfloat16* src = a.v + b * a.v_b + hkv * a.v_h + (int64_t)j * a.v_s + c;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float x = __bfloat162float(src[i]);
-        if (!(fabsf(x) <= 3.4e38f)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+      const __nv_bfloat16* src = a.v + b * a.v_b + hkv * a.v_h + (int64_t)j * a.v_s;
+#pragma unroll 1
+      for (int c = 0; c < HEAD_DIM; ++c) {
+        const float x = __bfloat162float(src[c]);
+        if (fabsf(x) <= 3.4e38f) continue;
+        if (part != nullptr)
+          part[c] += x;
+        else
+          out[c] = __float2bfloat16_rn(__bfloat162float(out[c]) + x);
       }
     }
   }
@@ -429,16 +436,26 @@ __device__ __forceinline__ void join_cluster(const WinArgs& a, uint32_t sbase, i
     int pos, head;
     if (!row_of(r, pos, head)) continue;
     PartSum sum;
-    bool any_nan = false;
-    for (int p = 0; p < PARTS * a.splits; ++p) {
-      const float2 ml = ld_cluster_f2(map_to_cta(sbase + L::ML + (p % PARTS * BLOCK_M + r) * 8, p / PARTS));
-      sum.top = fmaxf(sum.top, ml.x);
-      any_nan |= ml.y != ml.y;
-    }
-    for (int p = 0; p < PARTS * a.splits; ++p) {
-      const int slot = p % PARTS * BLOCK_M + r, cta = p / PARTS;
-      sum.add(ld_cluster_f2(map_to_cta(sbase + L::ML + slot * 8, cta)),
-              ld_cluster_f4(map_to_cta(sbase + (slot * L::PITCH + lane * 4) * 4, cta)));
+    // lane p has part p's maximum and sum (at most 16 parts)
+    const int parts = PARTS * a.splits;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < parts) ml = ld_cluster_f2(map_to_cta(sbase + L::ML + (lane % PARTS * BLOCK_M + r) * 8, lane / PARTS));
+    sum.top = ml.x;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) sum.top = fmaxf(sum.top, __shfl_xor_sync(0xffffffffu, sum.top, off));
+    sum.top = __shfl_sync(0xffffffffu, sum.top, 0);
+    const bool any_nan = __any_sync(0xffffffffu, ml.y != ml.y);
+#pragma unroll 1
+    for (int p0 = 0; p0 < parts; p0 += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p0 + i < parts)
+          x[i] = ld_cluster_f4(map_to_cta(sbase + (((p0 + i) % PARTS * BLOCK_M + r) * L::PITCH + lane * 4) * 4, (p0 + i) / PARTS));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p0 + i < parts)
+          sum.add(make_float2(__shfl_sync(0xffffffffu, ml.x, p0 + i), __shfl_sync(0xffffffffu, ml.y, p0 + i)), x[i]);
     }
     const float inv = any_nan ? __uint_as_float(0x7fc00000u) : row_inverse(a, sum.l, pos + n - a.Sq, n);
     reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Sq + pos) * a.H + head) * HEAD_DIM)[lane] = sum.row(inv);
@@ -742,6 +759,10 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (ok && warp_ok) {
         const float inv = row.sum != row.sum ? 1.0f : row_inverse(args, row.sum, min(pos, args.Sq - 1) + span.n - args.Sq, span.n);
         const int slot = t * BLOCK_M + r;
+        // where the row's part goes, null: the row is final
+        float* part = args.join ? reinterpret_cast<float*>(smem) + slot * L::PITCH
+                      : parts ? args.part_o + (it.split * args.total_rows + out_row) * HEAD_DIM
+                              : nullptr;
         if (row_ok) {
           const float2 ml = make_float2(row.top * args.scale_log2, row.sum);
           if (args.join)
@@ -750,7 +771,6 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             args.part_ml[it.split * args.total_rows + out_row] = ml;
         }
         __syncwarp();
-        const bool fix = *nonfinite != 0;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           uint32_t o[32];
@@ -766,17 +786,17 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::OE + t));
           }
-          if (fix && row_ok) add_nonfinite(args, span, row, 0, 1, steps, it.hkv, it.b, c, o);
           if (row_ok) {
-            if (args.join)
-              store_f32(reinterpret_cast<float*>(smem) + slot * L::PITCH + c, o);
-            else if (parts)
-              store_f32(args.part_o + (it.split * args.total_rows + out_row) * HEAD_DIM + c, o);
+            if (part != nullptr)
+              store_f32(part + c, o);
             else
               store_bf16(args.out + out_row * HEAD_DIM + c, o, inv);
           }
           __syncwarp();   // the next columns are loaded by the whole warp
         }
+        if (*nonfinite != 0 && row_ok)
+          add_nonfinite(args, span, row, 0, 1, steps, it.hkv, it.b, part, args.out + out_row * HEAD_DIM);
+        __syncwarp();
       } else if (steps > 0) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L::OE + t));
@@ -835,7 +855,22 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
+  const Item it = decode_item(args, blockIdx.x);
+  const Span span = make_span(args, 0, args.Sq, it.b, it.split);
+  const int steps = span.steps;
+  const int rows = args.Sq * args.pack;
+
+  // Loads first: the ring's first stages as soon as the barriers exist, Q into registers, so that
+  // memory works while tensor memory is allocated and the warps meet.
+  auto start_k = [&](int j) {
+    const int st = j % STAGES;
+    load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), step_key(span, j), it.hkv, it.b, args.k_swap);
+  };
+  auto start_v = [&](int j) {
+    const int st = j % STAGES;
+    load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), step_key(span, j), it.hkv, it.b, args.v_swap);
+  };
+  if (threadIdx.x == kLoadWarp * 32) {
     for (int i = 0; i < L::NUM; ++i) {
       int count = 1;
       if (i == L::QF || (i >= L::PF && i < L::KF)) count = 4;            // the tile's four warps
@@ -846,41 +881,63 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     *abort_flag = 0;
     *nonfinite = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tmap_k);
-    tma_prefetch_desc(&tmap_v);
+    fence_proxy_async_smem();
+    for (int j = 0; j < min(steps, STAGES); ++j) {
+      start_k(j);
+      start_v(j);
+    }
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
+  // the rows of Q: 16 lanes per row, 8 rows per pass
+  const int tid = threadIdx.x & 127, c16 = tid & 15;
+  uint4 qv[16];
+  if (warp < 4 && steps > 0) {
+#pragma unroll
+    for (int p = 0; p < 16; ++p) {
+      if (p * 8 < rows) {
+        const int r = min(p * 8 + (tid >> 4), rows - 1);
+        const int i = r / args.pack, h = it.h0 + r - i * args.pack;
+        qv[p] = ldg_stream(reinterpret_cast<const uint4*>(args.q + it.b * args.q_b + h * args.q_h + i * args.q_s) + c16);
+      }
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const Item it = decode_item(args, blockIdx.x);
-  const Span span = make_span(args, 0, args.Sq, it.b, it.split);
-  const int steps = span.steps;
+  // Rows past the last hold a copy of it up to the pass's end, and anything behind: they go nowhere.
+  if (warp < 4 && steps > 0) {
+#pragma unroll
+    for (int p = 0; p < 16; ++p) {
+      if (p * 8 < rows) {
+        const int r = p * 8 + (tid >> 4);
+        sts128(sbase + L::Q + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), qv[p]);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(L::QF));
+  }
 
   if (warp >= kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS_SERVICE));
     if (warp == kLoadWarp) {
       if (lane == 0) {
+        // The first stages are on their way.  A step's K is free long before its V (the streams' MMAs
+        // alternate), so K runs a step ahead: behind V it would wait for the other stream's product too.
         auto load_k = [&](int j) -> bool {
-          const int st = j % STAGES;
-          if (!wait(L::KE + st, (j / STAGES) ^ 1)) return false;
-          load_tile(sbase + L::K + st * TILE_BYTES, &tmap_k, bar(L::KF + st), step_key(span, j), it.hkv, it.b, args.k_swap);
+          if (!wait(L::KE + j % STAGES, (j / STAGES) ^ 1)) return false;
+          start_k(j);
           return true;
         };
-        auto load_v = [&](int j) -> bool {
-          const int st = j % STAGES;
-          if (!wait(L::VE + st, (j / STAGES) ^ 1)) return false;
-          load_tile(sbase + L::V + st * TILE_BYTES, &tmap_v, bar(L::VF + st), step_key(span, j), it.hkv, it.b, args.v_swap);
-          return true;
-        };
-        // A step's K is free long before its V (the streams' MMAs alternate), so K runs a step ahead:
-        // behind V it would wait for the other stream's product as well.
-        bool ok = steps == 0 || load_k(0);
-        for (int j = 0; ok && j < steps; ++j) ok = (j + 1 >= steps || load_k(j + 1)) && load_v(j);
+        bool ok = steps <= STAGES || load_k(STAGES);
+        for (int j = STAGES; ok && j < steps; ++j) {
+          ok = (j + 1 >= steps || load_k(j + 1)) && wait(L::VE + j % STAGES, (j / STAGES) ^ 1);
+          if (ok) start_v(j);
+        }
       }
     } else if (warp >= kFixWarp) {
       const int ft = threadIdx.x - kFixWarp * 32;
@@ -948,29 +1005,6 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FEW_REGS_SOFTMAX));
     const int t = warp >> 2;
     const int quarter = warp & 3;
-    const int rows = args.Sq * args.pack;
-    if (steps > 0 && t == 0) {
-      // the rows of Q: 16 lanes per row, all loads in flight before the first store
-      const int tid = threadIdx.x & 127, c16 = tid & 15;
-      uint4 v[16];
-#pragma unroll
-      for (int p = 0; p < 16; ++p) {
-        const int r = p * 8 + (tid >> 4);
-        v[p] = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-          const int i = r / args.pack, h = it.h0 + r - i * args.pack;
-          v[p] = ldg_stream(reinterpret_cast<const uint4*>(args.q + it.b * args.q_b + h * args.q_h + i * args.q_s) + c16);
-        }
-      }
-#pragma unroll
-      for (int p = 0; p < 16; ++p) {
-        const int r = p * 8 + (tid >> 4);
-        sts128(sbase + L::Q + (c16 >> 3) * HALF_BYTES + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), v[p]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::QF));
-    }
     const int uses = (steps + 1 - t) >> 1;   // steps of this stream
     const int r = quarter * 32 + lane;
     const bool row_ok = r < rows;
@@ -1008,6 +1042,9 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       const int64_t part_row = (2 * it.split + t) * args.total_rows + out_row;
       const float inv = row.sum != row.sum ? 1.0f : row_inverse(args, row.sum, pos + span.n - args.Sq, span.n);
       const int slot = t * BLOCK_M + r;
+      float* part = args.join ? reinterpret_cast<float*>(smem) + slot * L::PITCH
+                    : parts ? args.part_o + part_row * HEAD_DIM
+                            : nullptr;
       if (row_ok) {
         const float2 ml = make_float2(row.top * args.scale_log2, row.sum);
         if (args.join)
@@ -1016,7 +1053,6 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           args.part_ml[part_row] = ml;
       }
       __syncwarp();
-      const bool fix = *nonfinite != 0;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
         uint32_t o[32];
@@ -1027,17 +1063,17 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (fix && row_ok) add_nonfinite(args, span, row, t, 2, steps, it.hkv, it.b, c, o);
         if (row_ok) {
-          if (args.join)
-            store_f32(reinterpret_cast<float*>(smem) + slot * L::PITCH + c, o);
-          else if (parts)
-            store_f32(args.part_o + part_row * HEAD_DIM + c, o);
+          if (part != nullptr)
+            store_f32(part + c, o);
           else
             store_bf16(args.out + out_row * HEAD_DIM + c, o, inv);
         }
         __syncwarp();   // the next columns are loaded by the whole warp
       }
+      if (*nonfinite != 0 && row_ok)
+        add_nonfinite(args, span, row, t, 2, steps, it.hkv, it.b, part, args.out + out_row * HEAD_DIM);
+      __syncwarp();
     }
     if (args.join) {
       __syncwarp();
