@@ -289,6 +289,7 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
                                sf_tmem + SFB_COL + (k >> 1) * 8, (kb | k) != 0);
             commit_all<PAIR>(empty0 + stage * 8);
           }
+          __syncwarp();   // no lane falls a phase of a barrier behind the one that issues
           sbuf ^= 1;
           if (++back == STAGES) {
             back = 0;
@@ -514,6 +515,7 @@ mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                             sf_tmem + SFB_COL + (k >> 1) * 4, (kb > kb0 || k > 0) ? 1u : 0u);
         tc_commit(empty0 + stage * 8);
       }
+      __syncwarp();   // no lane falls a phase of a barrier behind the one that issues
       sbuf ^= 1;
       if (++back == S_STAGES) {
         back = 0;
