@@ -62,7 +62,8 @@ struct WinSmem {
   static constexpr int Q = 0;
   static constexpr int K = Q + (FEW ? 1 : 2) * TILE_BYTES;
   static constexpr int V = K + STAGES * TILE_BYTES;
-  static constexpr int NEXT = V + STAGES * TILE_BYTES;           // answers of the work scheduler (2 x 16)
+  static constexpr int OUT = V + STAGES * TILE_BYTES;            // rows on their way out, 4 KB per softmax warp
+  static constexpr int NEXT = OUT + (FEW ? 0 : kSoftmaxWarps * 4096);   // answers of the work scheduler (2 x 16)
   static constexpr int BARS = NEXT + 32;
   // barriers; [stage] or [tile], P by part and tile
   static constexpr int QF = 0, SF = 2, OF = 4;                   // Q, S, O are there
@@ -723,6 +724,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem_base + COL_S0 + t * 128 + lane_sel;
     const uint32_t o_tmem = tmem_base + COL_O0 + t * 128 + lane_sel;
+    const uint32_t out_stage = sbase + L::OUT + warp * 4096;
     int index = blockIdx.x, g = 0, full_items = 0;
     bool ok = true;
     for (int fetch = 0; index >= 0; ++fetch) {
@@ -771,28 +773,64 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             args.part_ml[it.split * args.total_rows + out_row] = ml;
         }
         __syncwarp();
+        const int64_t row0 = ((int64_t)it.b * args.Sq + pos0 + t * args.tile_pos) * args.H + it.h0;
+        // Rows leave through 4 KB of shared memory per warp, 128 bytes of each at a time: a thread holds
+        // a row, a store takes four (written from the registers, each 16 bytes of a warp are 32 lines of
+        // L1, one per clock).  Short loops: straight code of this length spends its time on fetching
+        // instructions, with the other tile's softmax in the same caches.
+        const int rel = row_ok ? row_pos * args.H + row_head : -1;
+        char* dst = (parts ? reinterpret_cast<char*>(args.part_o + (it.split * args.total_rows + row0) * HEAD_DIM)
+                           : reinterpret_cast<char*>(args.out + row0 * HEAD_DIM)) + (lane & 7) * 16;
+        const int pitch = parts ? HEAD_DIM * 4 : HEAD_DIM * 2;
+        const uint32_t line = out_stage + lane * 128;
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t o[32];
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t o[16];
           if (steps > 0) {
-            tmem_ld_32x32b_x32(o_tmem + c, o);
+            tmem_ld_32x32b_x16(o_tmem + c, o);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
+            for (int i = 0; i < 16; ++i) o[i] = 0u;
           }
-          if (c == 96 && steps > 0) {   // O is in registers: the next item's may be written
+          if (c == 112 && steps > 0) {   // O is in registers: the next item's may be written
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::OE + t));
           }
-          if (row_ok) {
-            if (part != nullptr)
-              store_f32(part + c, o);
-            else
-              store_bf16(args.out + out_row * HEAD_DIM + c, o, inv);
+          bool full = false;
+          if (part != nullptr) {
+            const bool staged = !args.join;
+            const uint32_t to = staged ? line : sbase + (t * BLOCK_M + r) * L::PITCH * 4 + c * 4;
+            const uint32_t chunk = staged ? (c >> 2) & 4 : 0, swz = staged ? lane & 7 : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sts128(to + (((chunk + i) ^ swz) << 4), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+            full = staged && (c & 16);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              sts128(line + ((((c >> 3) & 7) + i) ^ (lane & 7)) * 16,
+                     make_uint4(pack_bf16x2_rn(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
+                                pack_bf16x2_rn(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
+                                pack_bf16x2_rn(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
+                                pack_bf16x2_rn(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv)));
+            full = (c & 48) == 48;
           }
-          __syncwarp();   // the next columns are loaded by the whole warp
+          __syncwarp();
+          if (full) {
+#pragma unroll 1
+            for (int i = 0; i < 8; i += 2) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int src = 4 * (i + k) + (lane >> 3);
+                const uint4 v = lds128(out_stage + src * 128 + (((lane & 7) ^ (src & 7)) << 4));
+                const int to = __shfl_sync(0xffffffffu, rel, src);
+                if (to >= 0) *reinterpret_cast<uint4*>(dst + (int64_t)to * pitch) = v;
+              }
+            }
+            dst += 128;
+            __syncwarp();   // the next columns take their place
+          }
         }
         if (*nonfinite != 0 && row_ok)
           add_nonfinite(args, span, row, 0, 1, steps, it.hkv, it.b, part, args.out + out_row * HEAD_DIM);
