@@ -317,25 +317,29 @@ constexpr int WIN_EMU_MASK = 0x02;
 template <class Publish>
 __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t o_tmem, float sl2, int sinks, int key0,
                                              bool rescale, int lane, Publish publish) {
+  {
+    // visible columns: [first, last] and those before `sink`
+    const int last = row.key_last - key0, first = row.key_first - key0, sink = sinks - key0;
+    if (__builtin_expect(__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N)), 0)) {
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        const uint32_t seen = columns_below(last + 1 - c) & (~columns_below(first - c) | columns_below(sink - c));
+        uint32_t x[32];
+        tmem_ld_32x32b_x32(s_tmem + c, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!(seen & (1u << i))) x[i] = 0xff800000u;   // -inf
+        tmem_st_32x32b_x16(s_tmem + c, *reinterpret_cast<uint32_t(*)[16]>(&x[0]));
+        tmem_st_32x32b_x16(s_tmem + c + 16, *reinterpret_cast<uint32_t(*)[16]>(&x[16]));
+      }
+      tmem_wait_st();
+    }
+  }
   uint32_t s[128];
 #pragma unroll
   for (int c = 0; c < 128; c += 32) tmem_ld_32x32b_x32(s_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[c]));
   tmem_wait_ld();
-  {
-    // visible columns: [first, last] and those before `sink`
-    const int last = row.key_last - key0, first = row.key_first - key0, sink = sinks - key0;
-    if (__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N))) {
-      // a bit per visible column, 32 at a time: testing constant bits of a word costs a third of
-      // three comparisons per score
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t seen = columns_below(last + 1 - 32 * w) & (~columns_below(first - 32 * w) | columns_below(sink - 32 * w));
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (!(seen & (1u << i))) s[32 * w + i] = 0xff800000u;   // -inf
-      }
-    }
-  }
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 128; c += 2)
