@@ -620,8 +620,8 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         __syncwarp();
         if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
       }
-    } else {
-      const bool leader = elect_one() != 0;
+    } else if (elect_one() != 0) {
+      // One lane does it all: a lane that only waits could fall behind by a phase of a barrier.
       const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // tile 1: 128 columns on
       const uint32_t q0 = desc_lo(sbase + L::Q, 16);
       const uint32_t k0 = desc_lo(sbase + L::K, 16);
@@ -632,8 +632,8 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       bool ok = true;
       // S of tile t = Q . K^T of the stage's keys
       auto issue_qk = [&](int t, int st) {
-        if (leader) mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + t * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
-        if (leader) tc_commit(bar(L::SF + t));
+        mma_f16_ss_kmajor_x8(s0 + t * 128, q0 + t * TILE_UNITS, k0 + st * TILE_UNITS, kIdescQK);
+        tc_commit(bar(L::SF + t));
       };
       // O of tile t += P . V, each half of P as soon as it is published; `step` counts over all items
       auto issue_pv = [&](int t, int step, bool first) -> bool {
@@ -642,7 +642,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         for (int part = 0; part < 2; ++part) {
           if (!wait(L::PF + 2 * part + t, step)) return false;
           tc_fence_after();
-          if (leader) {
+          {
             if (part == 0)
               mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, first ? 0u : 1u);
             else
@@ -677,8 +677,8 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           if (!(ok = wait(L::QF + 1, full_items))) break;
           tc_fence_after();
           issue_qk(1, g & 1);
-          if (leader) tc_commit(bar(L::KE + (g & 1)));
-          if (steps == 1 && leader) tc_commit(bar(L::QE));
+          tc_commit(bar(L::KE + (g & 1)));
+          if (steps == 1) tc_commit(bar(L::QE));
           // the softmax warps have read the last item's O
           if (full_items > 0 && !(ok = wait(L::OE, full_items - 1) && wait(L::OE + 1, full_items - 1))) break;
           if (!(ok = wait_v(0))) break;
@@ -687,21 +687,21 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const bool last = j + 1 == steps;
             if (!(ok = issue_pv(0, g + j, j == 0))) break;
             if (last) {
-              if (leader) tc_commit(bar(L::OF));
+              tc_commit(bar(L::OF));
             } else {
               if (!(ok = wait_k(j + 1))) break;
               issue_qk(0, st ^ 1);
             }
             if (!(ok = issue_pv(1, g + j, j == 0))) break;
-            if (leader) tc_commit(bar(L::VE + st));
+            tc_commit(bar(L::VE + st));
             if (last) {
-              if (leader) tc_commit(bar(L::OF + 1));
+              tc_commit(bar(L::OF + 1));
             } else {
               // the next step's values, waited for while this step's MMAs are still queued
               if (!(ok = wait_v(j + 1))) break;
               issue_qk(1, st ^ 1);
-              if (leader) tc_commit(bar(L::KE + (st ^ 1)));
-              if (j + 2 == steps && leader) tc_commit(bar(L::QE));
+              tc_commit(bar(L::KE + (st ^ 1)));
+              if (j + 2 == steps) tc_commit(bar(L::QE));
             }
           }
           if (!ok) break;
@@ -709,8 +709,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           ++full_items;
         }
         index = next_item(fetch);
-        __syncwarp();
-        if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
+        if (more) mbar_arrive(bar(L::NE + (fetch & 1)));
       }
     }
     if (args.join) {   // the softmax warps' two meetings
@@ -995,8 +994,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L::VE + st));
       }
-    } else if (steps > 0) {
-      const bool leader = elect_one() != 0;
+    } else if (steps > 0 && elect_one() != 0) {   // one lane, as in window_tile_kernel
       const uint32_t s0 = tmem_base + COL_S0, o0 = tmem_base + COL_O0;   // stream 1: 128 columns on
       const uint32_t q0 = desc_lo(sbase + L::Q, 16);
       const uint32_t k0 = desc_lo(sbase + L::K, 16);
@@ -1008,11 +1006,9 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         const int st = j % STAGES, t = j & 1;
         if (!wait(L::KF + st, j / STAGES)) return false;
         tc_fence_after();
-        if (leader) {
-          mma_f16_ss_kmajor_x8(s0 + t * 128, q0, k0 + st * TILE_UNITS, kIdescQK);
-          tc_commit(bar(L::SF + t));
-          tc_commit(bar(L::KE + st));
-        }
+        mma_f16_ss_kmajor_x8(s0 + t * 128, q0, k0 + st * TILE_UNITS, kIdescQK);
+        tc_commit(bar(L::SF + t));
+        tc_commit(bar(L::KE + st));
         return true;
       };
       bool ok = wait(L::QF, 0) && issue_qk(0) && (steps == 1 || issue_qk(1));
@@ -1025,16 +1021,14 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         }
         if (!(ok = wait(L::PF + t, j >> 1))) break;
         tc_fence_after();
-        if (leader) mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, j > 1 ? 1u : 0u);
+        mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, j > 1 ? 1u : 0u);
         if (!(ok = wait(L::PF + 2 + t, j >> 1))) break;
         tc_fence_after();
-        if (leader) {
-          mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
-          tc_commit(bar(L::VE + st));
-        }
+        mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
+        tc_commit(bar(L::VE + st));
         if (j + 2 < steps)
           ok = issue_qk(j + 2);
-        else if (leader)
+        else
           tc_commit(bar(L::OF + t));
       }
     }
