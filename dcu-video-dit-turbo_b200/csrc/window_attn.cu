@@ -321,6 +321,10 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
     // visible columns: [first, last] and those before `sink`
     const int last = row.key_last - key0, first = row.key_first - key0, sink = sinks - key0;
     if (__builtin_expect(__any_sync(0xffffffffu, last < BLOCK_N - 1 || (first > 0 && sink < BLOCK_N)), 0)) {
+      // A bit per visible column, 32 at a time: testing constant bits of a word costs a third of three
+      // comparisons per score.  The masked scores go back to tensor memory: a short loop apart from the
+      // path that every step takes, against 128 more selects in it, takes 1 to 3 % less time (more with
+      // short windows), whole sequences included: the warps of both tiles run out of the instruction caches.
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
         const uint32_t seen = columns_below(last + 1 - c) & (~columns_below(first - c) | columns_below(sink - c));
@@ -787,37 +791,35 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int pitch = parts ? HEAD_DIM * 4 : HEAD_DIM * 2;
         const uint32_t line = out_stage + lane * 128;
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 16) {
-          uint32_t o[16];
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t o[32];
           if (steps > 0) {
-            tmem_ld_32x32b_x16(o_tmem + c, o);
+            tmem_ld_32x32b_x32(o_tmem + c, o);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0u;
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
-          if (c == 112 && steps > 0) {   // O is in registers: the next item's may be written
+          if (c == 96 && steps > 0) {   // O is in registers: the next item's may be written
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::OE + t));
           }
-          bool full = false;
+          bool full = !args.join;
           if (part != nullptr) {
-            const bool staged = !args.join;
-            const uint32_t to = staged ? line : sbase + (t * BLOCK_M + r) * L::PITCH * 4 + c * 4;
-            const uint32_t chunk = staged ? (c >> 2) & 4 : 0, swz = staged ? lane & 7 : 0;
+            const uint32_t to = full ? line : sbase + (t * BLOCK_M + r) * L::PITCH * 4 + c * 4;
+            const uint32_t swz = full ? lane & 7 : 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sts128(to + (((chunk + i) ^ swz) << 4), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
-            full = staged && (c & 16);
+            for (int i = 0; i < 8; ++i) sts128(to + ((i ^ swz) << 4), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
           } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4; ++i)
               sts128(line + ((((c >> 3) & 7) + i) ^ (lane & 7)) * 16,
                      make_uint4(pack_bf16x2_rn(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
                                 pack_bf16x2_rn(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
                                 pack_bf16x2_rn(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
                                 pack_bf16x2_rn(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv)));
-            full = (c & 48) == 48;
+            full = (c & 32) != 0;
           }
           __syncwarp();
           if (full) {
