@@ -105,7 +105,7 @@ struct WinArgs {
   const __nv_bfloat16* v;       // for the non-finite path
   const int* lengths;           // keys per sequence, null: Sk
   int64_t q_b, q_h, q_s, v_b, v_h, v_s;   // strides in elements
-  int H, share, Sq, Sk;                   // share = H / Hkv
+  int B, H, share, Sq, Sk;                // share = H / Hkv
   int pack, tile_pos, blocks;             // heads per row group; positions per tile; work items along positions
   int left, right, sinks, splits;
   int64_t total_rows;                     // B * Sq * H
@@ -113,6 +113,10 @@ struct WinArgs {
   float scale_log2;
 };
 
+// The last positions of a causal call see the most keys: those of all heads and sequences come first, so
+// that the SMs run out of work on short items.  Against head after head: 24 heads x 8192 causal 422 ->
+// 363 us, 2 x 24 heads x 4096 with a window of 1023 144 -> 135, none of 20 calls slower (keys of all heads
+// are in use at a time: 800 MB of them, causal, 3 % faster all the same).
 // One work item: positions [pos0, pos0 + CTA positions) of `pack` heads from h0, a share of their keys.
 struct Item {
   int split, block, h0, hkv, b;
@@ -121,9 +125,9 @@ __device__ __forceinline__ Item decode_item(const WinArgs& a, int index) {
   Item it;
   const int rest = index / a.splits;
   it.split = index - rest * a.splits;
-  const int heads = rest / a.blocks;
-  it.block = a.blocks - 1 - (rest - heads * a.blocks);   // the last positions of a causal call see the most keys: first
   const int groups = a.H / a.pack;
+  const int row = rest / (groups * a.B), heads = rest - row * groups * a.B;
+  it.block = a.blocks - 1 - row;
   it.b = heads / groups;
   it.h0 = (heads - it.b * groups) * a.pack;
   it.hkv = it.h0 / a.share;
@@ -1301,6 +1305,7 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   a.v_b = vs[0];
   a.v_h = vs[1];
   a.v_s = vs[2];
+  a.B = B;
   a.H = H;
   a.share = H / Hkv;
   a.Sq = Sq;
