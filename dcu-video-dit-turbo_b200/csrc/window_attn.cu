@@ -1144,25 +1144,63 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
 }
 
-// Joins the parts that lie in memory: one warp per row, four columns per lane.
+// Joins the parts that lie in memory: WARPS warps per row, four columns per lane.  Four parts at a time:
+// their loads are under way together, the first four's under the search for the maximum (one at a
+// time and one warp per row, 128 parts of a single row took 39 us more).
+template <int WARPS>
 __global__ void __launch_bounds__(256)
 window_join_kernel(const WinArgs args, int parts) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  __shared__ float4 sums[WARPS][32];
+  __shared__ float ls[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = WARPS > 1 ? warp * 4 : 0;   // this warp's parts: first .. first + 3, and so on
+  const int64_t row = WARPS > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
   if (row >= args.total_rows) return;
+  const float2* ml = args.part_ml + row;
+  const float4* o = reinterpret_cast<const float4*>(args.part_o) + row * (HEAD_DIM / 4) + lane;
+  float2 w[4];
+  float4 x[4];
+  auto load = [&](int p0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = min(p0 + i, parts - 1);
+      w[i] = ml[p * args.total_rows];
+      x[i] = o[p * args.total_rows * (HEAD_DIM / 4)];
+    }
+  };
+  load(first);
   PartSum sum;
   bool any_nan = false;
   for (int p = lane; p < parts; p += 32) {
-    const float2 ml = args.part_ml[p * args.total_rows + row];
-    sum.top = fmaxf(sum.top, ml.x);
-    any_nan |= ml.y != ml.y;
+    const float2 v = ml[p * args.total_rows];
+    sum.top = fmaxf(sum.top, v.x);
+    any_nan |= v.y != v.y;
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum.top = fmaxf(sum.top, __shfl_xor_sync(0xffffffffu, sum.top, off));
   any_nan = __any_sync(0xffffffffu, any_nan);
-  for (int p = 0; p < parts; ++p)
-    sum.add(args.part_ml[p * args.total_rows + row],
-            reinterpret_cast<const float4*>(args.part_o + (p * args.total_rows + row) * HEAD_DIM)[lane]);
+#pragma unroll 1
+  for (int p0 = first; p0 < parts;) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p0 + i < parts) sum.add(w[i], x[i]);
+    p0 += 4 * WARPS;
+    if (p0 < parts) load(p0);
+  }
+  if (WARPS > 1) {
+    sums[warp][lane] = sum.o;
+    if (lane == 0) ls[warp] = sum.l;
+    __syncthreads();
+    if (warp > 0) return;
+    for (int i = 1; i < WARPS; ++i) {
+      const float4 v = sums[i][lane];
+      sum.l += ls[i];
+      sum.o.x += v.x;
+      sum.o.y += v.y;
+      sum.o.z += v.z;
+      sum.o.w += v.w;
+    }
+  }
   const int64_t bi = row / args.H;
   const int b = (int)(bi / args.Sq), i = (int)(bi - (int64_t)b * args.Sq);
   const int n = sequence_keys(args.lengths, b, args.Sk);
@@ -1203,10 +1241,11 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
   // One CTA runs per SM, so a grid takes rounds of (its steps + a fixed part: set-up, first loads,
   // output).  The figures are microseconds measured on a B200 with 24, 48 and 96 CTAs before
   // splitting: a few-row step takes 0.83 alone and what 64 KB per CTA take from memory when many run; a
-  // full step 1.85.  A cluster joins its parts for one (few rows) or seven (256 rows), but leaves
+  // full step 1.85.  A cluster joins its parts for one (few rows) or nine (256 rows), but leaves
   // SMs without a place; parts in memory take a second kernel and 1040 bytes per row and part, there
-  // and back.  For 24 heads' single tokens over 8192 keys: 65.6 us unsplit, 32.8 in clusters of four,
-  // 35.8 in four parts through memory.
+  // and back.  24 heads' single tokens over 8192 keys: 65.5 us unsplit, 32.7 in clusters of four, 33.9 in
+  // four parts through memory; 24 x 300 rows over 8192 keys: 121 unsplit, 84 in clusters of two, 78.8 in
+  // two parts through memory, 62.5 in three; 2 heads x 700 over 16384: 49 in clusters of eight, 36 in 24 parts.
   constexpr int kSlots[kMaxCluster + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
   const int64_t ctas = (int64_t)p.blocks * (H / p.pack) * B;
   double best = 1e30;
@@ -1218,7 +1257,7 @@ WinPlan make_plan(int B, int H, int Hkv, int Sq, int Sk, int left, int right, in
     const double running = (double)(n < slots ? n : slots);
     const double step = p.few ? (running * 0.0109 > 0.83 ? running * 0.0109 : 0.83) : 1.85;
     double cost = rounds * ((double)steps / s * step + (p.few ? 8.0 : 5.0));
-    if (cluster && (s > 1 || p.few)) cost += p.few ? 1.0 : 7.0 * rounds;
+    if (cluster && (s > 1 || p.few)) cost += p.few ? 1.0 : 9.0 * rounds;
     if (!cluster) cost += 6.0 + 2.1e-4 * (double)((int64_t)Sq * H * B) * s * (p.few ? 2 : 1);
     if (cost < best) {
       best = cost;
@@ -1339,7 +1378,11 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
     return fail(B2_LAUNCH_FAILED, "window_fwd: launch failed: %s", cudaGetErrorString(e));
   }
   if (plan.parts == 1) return B2_OK;
-  window_join_kernel<<<(unsigned)((a.total_rows + 7) / 8), 256, 0, stream>>>(a, plan.parts);
+  // a block per row where a warp would read many parts in turn
+  if (plan.parts >= 16 && a.total_rows <= 8192)
+    window_join_kernel<8><<<(unsigned)a.total_rows, 256, 0, stream>>>(a, plan.parts);
+  else
+    window_join_kernel<1><<<(unsigned)((a.total_rows + 7) / 8), 256, 0, stream>>>(a, plan.parts);
   return check_launch("window_fwd (join)");
 }
 
