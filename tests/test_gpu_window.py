@@ -231,3 +231,13 @@ def test_refusals(cuda_pkg):
                         (lambda: f(q, torch.zeros((1, 2, 128, 32), dtype=torch.bfloat16, device=DEV).transpose(2, 3), v, SCALE, 1, 1), "contiguous last")]:
         with pytest.raises(RuntimeError, match=match):
             call()
+
+
+@pytest.mark.parametrize("B,H,Hkv", [(5, 27, 27), (5, 33, 11), (7, 39, 13)])
+def test_more_items_than_one_order_of_positions(cuda_pkg, B, H, Hkv):
+    """Row groups enough for two orders of positions one after the other and for three, the last of them
+    with fewer groups (of one head, of three)."""
+    q, k, v = qkv(B, H, Hkv, 2100, 2100, H)
+    lengths = torch.tensor([2100, 37, 1500, 0, 2099, 2100, 700], dtype=torch.int32, device=DEV)[:B].contiguous()
+    check(cuda_pkg, q, k, v, 130, 0, 4)
+    check(cuda_pkg, q, k, v, 130, 0, 4, lengths)
