@@ -241,3 +241,12 @@ def test_more_items_than_one_order_of_positions(cuda_pkg, B, H, Hkv):
     lengths = torch.tensor([2100, 37, 1500, 0, 2099, 2100, 700], dtype=torch.int32, device=DEV)[:B].contiguous()
     check(cuda_pkg, q, k, v, 130, 0, 4)
     check(cuda_pkg, q, k, v, 130, 0, 4, lengths)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk", [(1, 2, 2, 700, 700), (2, 6, 2, 1100, 900), (1, 4, 1, 3, 600), (2, 31, 31, 1300, 1300)])
+@pytest.mark.parametrize("left,sinks", [(0, 0), (100, 3), (500, 0)])
+def test_a_limit_behind_and_none_ahead(cuda_pkg, B, H, Hkv, Sq, Sk, left, sinks):
+    """The first positions see the most keys."""
+    q, k, v = qkv(B, H, Hkv, Sq, Sk, Sq + left)
+    check(cuda_pkg, q, k, v, left, -1, sinks)
+    check(cuda_pkg, q, k, v, left, -1, sinks, torch.tensor([Sk // 3, Sk], dtype=torch.int32, device=DEV)[:B].contiguous())
