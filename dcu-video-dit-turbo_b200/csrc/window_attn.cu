@@ -350,8 +350,26 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
       // comparisons per score.  The masked scores go back to tensor memory: a short loop apart from the
       // path that every step takes, against 128 more selects in it, takes 1 to 3 % less time (more with
       // short windows), whole sequences included: the warps of both tiles run out of the instruction caches.
+      // A tile that no row of the warp sees (a step is the CTA's, its last rows see other keys than its
+      // first) has P = 0 and leaves the exp2 unit to the other warps: 2 to 6 % with windows up to 511.
+      if (__all_sync(0xffffffffu, last < 0 || (first >= BLOCK_N && sink <= 0))) {
+        const uint32_t zero[16] = {};
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) tmem_st_32x32b_x16(s_tmem + c, zero);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          publish(0);
+          publish(1);
+        }
+        return;
+      }
+      // from the first column that some row of the warp does not see to the last
+      const int lo = __reduce_min_sync(0xffffffffu, min(first > 0 ? max(sink, 0) : 128, last + 1));
+      const int hi = __any_sync(0xffffffffu, last < BLOCK_N - 1) ? 128 : __reduce_max_sync(0xffffffffu, first);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = max(lo, 0) & ~31; c < min(hi, 128); c += 32) {
         const uint32_t seen = columns_below(last + 1 - c) & (~columns_below(first - c) | columns_below(sink - c));
         uint32_t x[32];
         tmem_ld_32x32b_x32(s_tmem + c, x);
@@ -375,6 +393,8 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
     mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
   const float m_row = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
   const bool raise = row.live && (m_row - row.top) * sl2 > 8.0f;   // false while both are -inf (NaN)
+  // a row that had seen nothing has added zeros to O so far (its values were cleared): nothing to rescale
+  const bool correct = raise && rescale && row.top != -INFINITY;
   float alpha = 1.0f;
   if (raise) {
     alpha = ex2_approx((row.top - m_row) * sl2);
@@ -382,7 +402,7 @@ __device__ __forceinline__ void softmax_step(Row& row, uint32_t s_tmem, uint32_t
     row.sum *= alpha;
   }
   __syncwarp();
-  if (rescale && __any_sync(0xffffffffu, raise)) {
+  if (__any_sync(0xffffffffu, correct)) {
 #pragma unroll 1
     for (int c = 0; c < 128; c += 16) {
       uint32_t o[16];
