@@ -55,8 +55,8 @@ constexpr int TILE_REGS_SOFTMAX = 216, TILE_REGS_SERVICE = 72;
 constexpr int FEW_REGS_SOFTMAX = 232, FEW_REGS_SERVICE = 40;
 static_assert(2 * TILE_REGS_SOFTMAX + TILE_REGS_SERVICE <= 3 * kLaunchRegs && 2 * FEW_REGS_SOFTMAX + FEW_REGS_SERVICE <= 3 * kLaunchRegs,
               "register split exceeds the CTA's launch allocation");
-// Shared memory: Q, the K ring, the V ring, barriers.  The few-row form has one tile of Q and a third
-// stage in its place.
+// Shared memory: Q, the K ring, the V ring, rows on their way out, barriers.  The few-row form has one tile
+// of Q and a third stage in its place, and none of the rows.
 template <bool FEW>
 struct WinSmem {
   static constexpr int STAGES = FEW ? 3 : 2;
@@ -121,7 +121,7 @@ struct WinArgs {
   int64_t q_b, q_h, q_s, v_b, v_h, v_s;   // strides in elements
   int H, share, groups, Sq, Sk;           // share = H / Hkv, groups = H / pack
   int together, last, chunks;             // row groups whose items are in order; in the last chunk; chunks
-  int first_first;                        // the first positions see the most keys
+  int ascending;                          // the first positions see the most keys
   Divisor by_splits, by_chunk, by_together, by_last, by_groups, by_share;
   int pack, tile_pos, blocks;             // heads per row group; positions per tile; work items along positions
   int left, right, sinks, splits;
@@ -149,7 +149,7 @@ __device__ __forceinline__ Item decode_item(const WinArgs& a, int index) {
   const bool last = chunk == a.chunks - 1;
   const int row = quotient(in, last ? a.by_last : a.by_together);
   const int heads = chunk * a.together + in - row * (last ? a.last : a.together);
-  it.block = a.first_first ? row : a.blocks - 1 - row;
+  it.block = a.ascending ? row : a.blocks - 1 - row;
   it.b = quotient(heads, a.by_groups);
   it.h0 = (heads - it.b * a.groups) * a.pack;
   it.hkv = quotient(it.h0, a.by_share);
@@ -592,7 +592,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const uint32_t tmem_base = *tmem_slot;
   const int item_pos = 2 * args.tile_pos;
 
-  // The item after `fetch` others, or -1.  Called by whole warps (the loader by one lane) in step.
+  // The item after `fetch` others, or -1.  Called by whole warps in step, by one lane of those that load and issue.
   auto next_item = [&](int fetch) -> int {
     if (!more) return -1;
     const int slot = fetch & 1;
@@ -692,12 +692,10 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         for (int part = 0; part < 2; ++part) {
           if (!wait(L::PF + 2 * part + t, step)) return false;
           tc_fence_after();
-          {
-            if (part == 0)
-              mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, first ? 0u : 1u);
-            else
-              mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
-          }
+          if (part == 0)
+            mma_f16_ts_seq<0, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, first ? 0u : 1u);
+          else
+            mma_f16_ts_seq<4, 4>(o0 + t * 128, s0 + t * 128, v0 + st * TILE_UNITS, kIdescPV, 1u);
         }
         return true;
       };
@@ -1392,7 +1390,7 @@ int launch_window_fwd(const void* q, const void* k, const void* v, void* out, vo
   const int64_t least = left < 0 && right < 0 ? 1 : (4 * kNumSMsB200 + plan.blocks - 1) / plan.blocks;
   const int64_t chunks = all > least ? all / least : 1, together = (all + chunks - 1) / chunks;
   a.together = (int)together;
-  a.first_first = left >= 0 && right < 0 ? 1 : 0;
+  a.ascending = left >= 0 && right < 0 ? 1 : 0;
   a.chunks = (int)((all + together - 1) / together);
   a.last = (int)(all - (a.chunks - 1) * together);
   a.groups = H / plan.pack;
