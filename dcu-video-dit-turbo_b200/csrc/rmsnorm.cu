@@ -8,8 +8,10 @@
 // Bound by memory: 4 bytes in and 2 + 1 (2 + 17/32) bytes out per element.  A row is held by TPR
 // threads in registers from its only read to its quantised write; y is never rounded to bf16 in
 // between.  A thread keeps the same columns of every row, so the weight is read once per CTA.
-// Measured: int8 109099 x 3072 369 us = 6.36 TB/s, 23638 x 3072 86 us = 5.9; MXFP4 356 and 84 us.
-// The int8 scale divides by the fp32 scale that is stored, so q * scale is within half a step of y.
+// Measured: int8 109099 x 3072 378 us = 6.2 TB/s, 23638 x 3072 88 us = 5.8; MXFP4 361 and 85 us.
+// Roundings: the mean, 1 / sqrt, max|y| / 127 and y / scale are each rounded once, to the nearest fp32
+// (0 to 3 % more time than products with rounded reciprocals and the fast 1 / sqrt, 5 % at 16384 columns).
+// The elements divide by the fp32 scale that is stored, so q * scale is within half a step of y.
 #include "b2_common.cuh"
 #include "b2_launch.h"
 #include "mxfp4.cuh"
@@ -28,19 +30,40 @@ struct RmsArgs {
   void* scale;             // fp32 [M] or scale tiles
   int64_t M;
   int cvec;                // C / 8
-  float inv_c, eps;
+  double inv_c;            // 1 / C
+  float eps;
 };
 
-// What a row's int8 scale and multiplier are, from the row's largest magnitude.  Rows with a NaN or
-// an infinity keep that in the scale and get zero elements.
-__device__ __forceinline__ float int8_scale(float absmax, float& inv, bool& zero_row) {
-  float s = absmax != absmax ? absmax : fmaxf(__fmul_rn(absmax, kInv127), 1.0e-30f);
-  zero_row = !(s <= 3.4028234e38f);
-  inv = __frcp_rn(s);
-  return s;
+// v / n rounded to the nearest fp32, inv_n = 1 / n in 64 bits: a quotient of two 24-bit numbers is no
+// nearer to the middle between two fp32 than 2^-49 of itself, and the product is within 2^-52.
+__device__ __forceinline__ float quotient(float v, double inv_n) { return (float)((double)v * inv_n); }
+// 1 / sqrt(sum of squares / C + eps)
+__device__ __forceinline__ float row_rstd(float ss, double inv_c, float eps) {
+  return __frsqrt_rn(__fadd_rn(quotient(ss, inv_c), eps));
 }
-// Round half even of a value within +-127 (a few units in the last place over): low byte of the sum.
-__device__ __forceinline__ uint32_t int8_bits(float v) { return __float_as_uint(v + 12582912.0f) & 0xffu; }
+// A row's int8 scale, from its largest magnitude, and 1 / scale as a sum of two fp32.  Rows with a NaN or an
+// infinity keep that in the scale and get zero elements.
+struct Int8Scale {
+  float s, inv, inv_low;
+  bool zero_row;
+  __device__ __forceinline__ explicit Int8Scale(float absmax) {
+    s = absmax != absmax ? absmax : fmaxf(quotient(absmax, 1.0 / 127.0), 1.0e-30f);
+    zero_row = !(s <= 3.4028234e38f);
+    inv = __frcp_rn(s);
+    inv_low = fmaf(-s, inv, 1.0f) * inv;
+  }
+  // Round half even of y / s for a pair, |y| <= 127 s (a unit in the last place over): the low bytes of
+  // the sums.  The quotient is rounded once, to the nearest fp32: with the reciprocal's first part
+  // alone it put 4 to 6 of 1000 exact ties on the wrong side.
+  __device__ __forceinline__ void bits2(float y0, float y1, uint32_t& b0, uint32_t& b1) const {
+    const uint64_t y = pack2(y0, y1);
+    const uint64_t t = fma2(y, pack2(inv, inv), mul2(y, pack2(inv_low, inv_low)));
+    float e0, e1;
+    unpack2(add2(t, pack2(12582912.0f, 12582912.0f)), e0, e1);   // 1.5 * 2^23: nearest integer, ties to even
+    b0 = __float_as_uint(e0) & 0xffu;
+    b1 = __float_as_uint(e1) & 0xffu;
+  }
+};
 
 // Asks the vectors v0 .. v0 + vecs of x and residual into L2, one request per 128-byte line.
 template <int TPR, int VPT>
@@ -112,7 +135,7 @@ rmsnorm_residual_kernel(const RmsArgs a) {
     // consecutive reductions use the two buffers in turn
     const float ss = slot_allreduce<THREADS, TPR>((a0 + a1) + (b0 + b1), red[turn], slot, SumOp());
     turn ^= 1;
-    const float rstd = rsqrtf(ss * a.inv_c + a.eps);
+    const float rstd = row_rstd(ss, a.inv_c, a.eps);
     const uint64_t rstd2 = pack2(rstd, rstd);
     float y[VPT][8];
     uint32_t most = 0;
@@ -144,20 +167,18 @@ rmsnorm_residual_kernel(const RmsArgs a) {
       // maximum, but for a NaN that the row's own columns have as well
       const float absmax = slot_allreduce<THREADS, TPR>(__uint_as_float(most), red[turn], slot, NanMaxOp());
       turn ^= 1;
-      float inv;
-      bool zero_row;
-      const float s = int8_scale(absmax, inv, zero_row);
+      const Int8Scale scale(absmax);
       if (live) {
-        if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = s;
+        if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = scale.s;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const int c = lane + i * TPR;
           if (c < a.cvec) {
             uint2 o = make_uint2(0, 0);
-            if (!zero_row) {
+            if (!scale.zero_row) {
               uint32_t b[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) b[j] = int8_bits(y[i][j] * inv);
+              for (int j = 0; j < 8; j += 2) scale.bits2(y[i][j], y[i][j + 1], b[j], b[j + 1]);
               o.x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
               o.y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
             }
@@ -173,7 +194,7 @@ rmsnorm_residual_kernel(const RmsArgs a) {
 // residual, sum and q all start a row at the same place in theirs, so a row is held as the aligned
 // vectors that it touches: those at its two ends are shared with its neighbours and are stored
 // element by element.  The weight sits differently under every row and is read from shared memory.
-// Bound by instructions (a predicate and a two-byte load per element): 3.1 TB/s at 23638 x 1001 and
+// Bound by instructions (a predicate and a two-byte load per element): 2.9 TB/s at 23638 x 1001 and
 // 2.5 at 8192 x 4099; one CTA per row and two bytes per load reach 1.2 and 2.0.
 template <int THREADS, int TPR, int VPT>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS)
@@ -247,7 +268,7 @@ rmsnorm_residual_quant_odd_kernel(const RmsArgs a, const __nv_bfloat16* __restri
       }
     }
     ss = slot_allreduce<THREADS, TPR>(ss, red[0], slot, SumOp());
-    const float rstd = rsqrtf(ss * a.inv_c + a.eps);
+    const float rstd = row_rstd(ss, a.inv_c, a.eps);
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -259,18 +280,18 @@ rmsnorm_residual_quant_odd_kernel(const RmsArgs a, const __nv_bfloat16* __restri
         most = max(most, __float_as_uint(y[i][j]) & 0x7fffffffu);
       }
     const float absmax = slot_allreduce<THREADS, TPR>(__uint_as_float(most), red[1], slot, NanMaxOp());
-    float inv;
-    bool zero_row;
-    const float s = int8_scale(absmax, inv, zero_row);
+    const Int8Scale by(absmax);
     if (!live) continue;
-    if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = s;
+    if (lane == 0) reinterpret_cast<float*>(a.scale)[row] = by.s;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = lane + i * TPR;
       if (c >= vecs) break;
-      uint32_t b[8];
+      uint32_t b[8] = {};
+      if (!by.zero_row) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = zero_row ? 0u : int8_bits(y[i][j] * inv);
+        for (int j = 0; j < 8; j += 2) by.bits2(y[i][j], y[i][j + 1], b[j], b[j + 1]);
+      }
       uint2* dst = reinterpret_cast<uint2*>(a.q) + v0 + c;
       if (c * 8 >= head && c * 8 + 8 - head <= C) {
         *dst = make_uint2(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24), b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24));
@@ -291,7 +312,7 @@ __global__ void __launch_bounds__(kThreads)
 rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ residual,
                                       const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ sum,
                                       int8_t* __restrict__ q, float* __restrict__ scale, int64_t M, int64_t C,
-                                      float inv_c, float eps) {
+                                      double inv_c, float eps) {
   __shared__ float red[2][kThreads / 32];
   for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
     const int64_t at = row * C;
@@ -306,17 +327,18 @@ rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const
       ss = fmaf(v, v, ss);
     }
     ss = slot_allreduce<kThreads, kThreads>(ss, red[0], 0, SumOp());
-    const float rstd = rsqrtf(ss * inv_c + eps);
+    const float rstd = row_rstd(ss, inv_c, eps);
     uint32_t most = 0;
     for (int64_t c = threadIdx.x; c < C; c += kThreads)
       most = max(most, __float_as_uint(value(c) * rstd * __bfloat162float(weight[c])) & 0x7fffffffu);
     const float absmax = slot_allreduce<kThreads, kThreads>(__uint_as_float(most), red[1], 0, NanMaxOp());
-    float inv;
-    bool zero_row;
-    const float s = int8_scale(absmax, inv, zero_row);
-    if (threadIdx.x == 0) scale[row] = s;
-    for (int64_t c = threadIdx.x; c < C; c += kThreads)
-      q[at + c] = zero_row ? (int8_t)0 : (int8_t)int8_bits(value(c) * rstd * __bfloat162float(weight[c]) * inv);
+    const Int8Scale by(absmax);
+    if (threadIdx.x == 0) scale[row] = by.s;
+    for (int64_t c = threadIdx.x; c < C; c += kThreads) {
+      uint32_t bits = 0, other;
+      if (!by.zero_row) by.bits2(value(c) * rstd * __bfloat162float(weight[c]), 0.f, bits, other);
+      q[at + c] = (int8_t)bits;
+    }
   }
 }
 
@@ -324,7 +346,6 @@ rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const
 
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* sum, void* q, void* scale,
                             int64_t M, int64_t C, float eps, bool mx, cudaStream_t stream) {
-  const float inv_c = (float)(1.0 / (double)C);
   const bool aligned = aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(sum) &&
                        (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
   const bool vector = C % 8 == 0 && C <= 16384 && aligned;
@@ -333,7 +354,7 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
     const int64_t cap = (int64_t)kNumSMsB200 * 8;
     rmsnorm_residual_quant_generic_kernel<<<(unsigned)(M < cap ? M : cap), kThreads, 0, stream>>>(
         (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)weight, (__nv_bfloat16*)sum,
-        (int8_t*)q, (float*)scale, M, C, inv_c, eps);
+        (int8_t*)q, (float*)scale, M, C, 1.0 / (double)C, eps);
     return check_launch("rmsnorm_residual_quant");
   }
   RmsArgs a;
@@ -345,7 +366,7 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
   a.scale = scale;
   a.M = M;
   a.cvec = (int)(C / 8);
-  a.inv_c = inv_c;
+  a.inv_c = 1.0 / (double)C;
   a.eps = eps;
   if (!vector) {
 #define B2_RMS_ODD(THREADS, TPR, VPT)                                                                            \
