@@ -23,7 +23,7 @@ constexpr int kPasses = kMxTileRows / kRowsPerPass;         // 8
 
 // silu(g) * u = g / (1 + 2^(-g log2 e)) * u of a pair, in fp32 with the fast exponential and
 // reciprocal (a few units in the last place, five decimal digits below the step of the 4-bit
-// elements).  Below about -87 the reciprocal is flushed to zero: products under 1e-36 vanish.
+// elements).  Holds for g >= kFarGate: below -87 the reciprocal is flushed to zero.
 __device__ __forceinline__ uint64_t silu_mul2(uint64_t g, uint64_t u) {
   float x0, x1;
   unpack2(mul2(g, pack2(-1.4426950408889634f, -1.4426950408889634f)), x0, x1);
@@ -33,6 +33,16 @@ __device__ __forceinline__ uint64_t silu_mul2(uint64_t g, uint64_t u) {
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x0));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x1));
   return mul2(mul2(g, pack2(x0, x1)), u);
+}
+
+// Gates below it are rare (silu there is above -1.5e-33), but their product with a large `up` is not
+// zero: 2^-129, half the smallest element, is reached down to g = -183.  e^g = (e^(g/4))^4 times g and u one
+// after another, so no factor is flushed before the product is (1 + e^g is 1 here).
+constexpr float kFarGate = -80.0f;
+constexpr uint32_t kFarGateBits = 0xc2a0u;                  // in bf16; larger ones are further, -infinity or NaN
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+  const float e = expf(0.25f * g);
+  return g * e * u * e * e * e;
 }
 
 // A stage is 32 KB: a whole tile's rows, or with SwiGLU half of them, gate and up.
@@ -109,8 +119,9 @@ quantize_mxfp4_kernel(const __grid_constant__ CUtensorMap tmap, uint32_t* __rest
       // after a timeout every thread still walks its tiles (and meets the barriers), without waiting
       if (ok) ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout);
       const uint4* src = reinterpret_cast<const uint4*>(smem + stage * kStageBytes) + row_in_pass * 16 + lane16;
-#pragma unroll
-      for (int pp = 0; pp < PART_PASSES; ++pp) {
+      uint32_t gates = 0;                                   // the furthest gate's bits, in halves
+      // pass pp: this lane's eight columns of a row; `far` where some gates of the warp's rows are
+      auto pass = [&](int pp, bool far) {
         const int p = part * PART_PASSES + pp;
         const uint4 v = src[pp * kRowsPerPass * 16];
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -122,6 +133,15 @@ quantize_mxfp4_kernel(const __grid_constant__ CUtensorMap tmap, uint32_t* __rest
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             unpack2(silu_mul2(bf16x2_to_f32x2(w[i]), bf16x2_to_f32x2(uw[i])), f[2 * i], f[2 * i + 1]);
+          if (far) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float g = (i & 1) ? bf16hi_to_f32(w[i >> 1]) : bf16lo_to_f32(w[i >> 1]);
+              if (g < kFarGate) f[i] = silu_mul_far(g, (i & 1) ? bf16hi_to_f32(uw[i >> 1]) : bf16lo_to_f32(uw[i >> 1]));
+            }
+          } else {
+            gates = __vmaxu2(gates, __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3])));
+          }
           m = col < K ? mx_absmax_halves(f) : 0u;           // past the gate columns lie up columns, not zeros
         } else {
 #pragma unroll
@@ -132,6 +152,16 @@ quantize_mxfp4_kernel(const __grid_constant__ CUtensorMap tmap, uint32_t* __rest
         const uint32_t word = mx_gather_word(byte);
         if (p * kRowsPerPass < rows_left) dst[(int64_t)p * kRowsPerPass * (K / 8)] = mx_quantize8(f, byte);
         if (lane16 == 0) tile[mx_scale_offset(p * kRowsPerPass + row_in_pass, 0) / 4] = word;
+      };
+#pragma unroll
+      for (int pp = 0; pp < PART_PASSES; ++pp) pass(pp, false);
+      if constexpr (SWIGLU) {
+        // far gates are rare: the warp's rows are then done again, so that the passes above have no branch
+        // (with one in each, 109099 x 3072 took 267 us)
+        if (__any_sync(0xffffffffu, col < K && max(gates & 0xffffu, gates >> 16) > kFarGateBits)) {
+#pragma unroll 1
+          for (int pp = 0; pp < PART_PASSES; ++pp) pass(pp, true);
+        }
       }
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + stage * 8);
