@@ -798,11 +798,15 @@ def rmsnorm_residual_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weigh
 # ---- attention with a sliding window (no counterpart in the reference) --------------
 
 @functools.lru_cache(maxsize=1024)
-def _window_workspace(*sizes: int) -> int:
-    """Workspace bytes of a windowed attention call: a function of its sizes alone."""
+def _workspace_of(lib, *sizes: int) -> int:
     need = ctypes.c_int64(0)
-    _lib.check(_lib.load().b2_window_fwd_workspace(*sizes, ctypes.byref(need)), "b2_window_fwd_workspace")
+    _lib.check(lib.b2_window_fwd_workspace(*sizes, ctypes.byref(need)), "b2_window_fwd_workspace")
     return need.value
+
+
+def _window_workspace(*sizes: int) -> int:
+    """Workspace bytes of a windowed attention call: a function of its sizes alone, for one library."""
+    return _workspace_of(_lib.current(), *sizes)
 
 
 def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, left: int, right: int,
