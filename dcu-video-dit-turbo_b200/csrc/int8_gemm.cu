@@ -185,7 +185,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
     uint32_t buf_phase = 0;
     const EpilogueArgs& epi = args.epi;
     const bool fused = epi.out_i32 == nullptr;
-    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
+    bool ok = true;   // after a timeout a warp still walks its tiles (and meets the others), without waiting
+    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x, buf ^= 1, buf_phase ^= buf ^ 1) {
       int m_idx, n_idx;
       decode_tile(tile, args, m_idx, n_idx);
       const int col0 = n_idx * BN;
@@ -196,7 +197,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
         epilogue_stage_columns(epi, cvec, col0, et);
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
-      if (!mbar_wait(tfull0 + buf * 8, buf_phase, abort_flag, kStatusGemmTimeout)) break;
+      if (ok) ok = mbar_wait_warp(tfull0 + buf * 8, buf_phase, abort_flag, kStatusGemmTimeout);
+      if (!ok) continue;
       tc_fence_after();
       const bool row_ok = row < epi.M;
       const float rsv = (fused && row_ok) ? epi.rs[row] : 0.f;
@@ -232,8 +234,6 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(tempty0 + buf * 8);
-      buf ^= 1;
-      if (buf == 0) buf_phase ^= 1;
     }
   }
 

@@ -312,7 +312,8 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
     uint32_t buf_phase = 0;
     const uint32_t stage = ring + L::OUT + quarter * kEpiStageBytes;
     const uint32_t tfree_leader = PAIR ? map_to_cta(tfree, 0) : tfree;
-    for (int tile = first_tile; tile < args.num_tiles; tile += tile_step) {
+    bool ok = true;   // after a timeout a warp still walks its tiles (and meets the others), without waiting
+    for (int tile = first_tile; tile < args.num_tiles; tile += tile_step, buf ^= 1, buf_phase ^= buf ^ 1) {
       int m_idx, n_idx;
       decode_tile(tile, args, m_idx, n_idx);
       const int col0 = n_idx * BN;
@@ -327,7 +328,8 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
         bias[c] = b;
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (!mbar_wait(tfull0 + buf * 8, buf_phase, abort_flag, kStatusGemmTimeout)) break;
+      if (ok) ok = mbar_wait_warp(tfull0 + buf * 8, buf_phase, abort_flag, kStatusGemmTimeout);
+      if (!ok) continue;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (buf ? ACC1 : 0) + ((uint32_t)(quarter * 32) << 16);
       // the columns shared with the other accumulator come first: the last 64 of the first one,
@@ -368,8 +370,6 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
           bulk_commit_group();
         }
       }
-      buf ^= 1;
-      if (buf == 0) buf_phase ^= 1;
     }
     if (lane == 0) bulk_wait_group<0>();   // this warp's stores are complete before the CTA may retire
   }

@@ -89,6 +89,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
   return mbar_give_up(abort_flag, code);
 }
+// The wait of a whole warp that goes on together: all lanes have the same answer, and none is still in
+// it when another goes on.  Lanes that wait each for themselves can disagree on a timeout (the one
+// that leaves never meets the others at their next warp-wide instruction), and a lane that only
+// waits can fall behind the one that issues by a phase of the barrier, which then looks as if it
+// were still to come.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                               unsigned int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
+}
 
 // ---- TMA (tiled bulk tensor loads, no multicast) ----------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
