@@ -221,6 +221,7 @@ __device__ __forceinline__ void softmax_role(const FlashArgs& args, uint32_t tme
   }
   // ---- final: O / l -> bf16 -> global (BSHD) ----
   if (ok) ok = mbar_wait(bar(O_FULL + t), 0, abort_flag, kStatusFlashTimeout);
+  ok = __all_sync(0xffffffffu, ok);   // the warp goes on as one
   if (ok) {
     tc_fence_after();
     const float l = row_sum;

@@ -243,7 +243,8 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
   } else if (warp == 1) {
     if (rank == 0) {
       // The whole warp walks the loop and one elected lane issues: without a lane-divergent region
-      // around them, addresses and descriptors stay warp-uniform.
+      // around them, addresses and descriptors stay warp-uniform.  A lane whose wait gave up walks on
+      // without waiting: every lane meets the others after each stage, or none would get past it.
       const bool leader = elect_one() != 0;
       int stage = 0;
       uint32_t phase = 0;
@@ -253,10 +254,10 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
       bool first = true, ok = true;
       int back = STAGES - 2;   // ring position of two stages ago, and the parity of its release
       uint32_t back_phase = 1;
-      for (int tile = first_tile; ok && tile < args.num_tiles; tile += tile_step) {
+      for (int tile = first_tile; tile < args.num_tiles; tile += tile_step) {
         // the tile before must have left the columns that this one's accumulator shares with it
         if (!first) {
-          if (!(ok = mbar_wait(tfree, fphase, abort_flag, kStatusGemmTimeout))) break;
+          if (ok) ok = mbar_wait(tfree, fphase, abort_flag, kStatusGemmTimeout);
           fphase ^= 1;
           tc_fence_after();
         }
@@ -264,8 +265,8 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
         const uint32_t d_tmem = tmem_base + (buf ? ACC1 : 0);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           // the stage is filled, and the MMAs that used this scale buffer (two stages ago) are done
-          if (!(ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout))) break;
-          if (!(ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout))) break;
+          if (ok) ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout);
+          if (ok) ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout);
           tc_fence_after();
           const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
           const uint32_t sf = ring + L::SF + stage * SF_STAGE;
@@ -273,7 +274,7 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
           const uint32_t a_addr = ring + stage * L::STAGE_BYTES;
           const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
           const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
-          if (leader) {
+          if (leader && ok) {
             // [k tile][row group of 32]: 4 columns of A per k tile, 8 of W
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
@@ -300,8 +301,7 @@ __device__ __forceinline__ void mxfp4_gemm_body(const CUtensorMap& tmap_a, const
             phase ^= 1;
           }
         }
-        if (!ok) break;
-        if (leader) commit_all<PAIR>(tfull0 + buf * 8);
+        if (leader && ok) commit_all<PAIR>(tfull0 + buf * 8);
         buf ^= 1;
       }
     }
@@ -493,8 +493,8 @@ mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     uint32_t back_phase = 1;
     bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!(ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout))) break;
-      if (!(ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout))) break;
+      if (ok) ok = mbar_wait(full0 + stage * 8, phase, abort_flag, kStatusGemmTimeout);
+      if (ok) ok = mbar_wait(empty0 + back * 8, back_phase, abort_flag, kStatusGemmTimeout);
       tc_fence_after();
       const int steps = min(BKE / UMMA_K, (args.K - kb * BKE + UMMA_K - 1) / UMMA_K);
       const uint32_t sf = ring + S_SF + stage * S_SF_STAGE;
@@ -502,7 +502,7 @@ mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       const uint32_t a_addr = ring + stage * S_STAGE_BYTES;
       const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
       const uint64_t bdesc = make_smem_desc_sw128(a_addr + A_BYTES, 16, 1024);
-      if (leader) {
+      if (leader && ok) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           scales_to_tmem<false>(sf_tmem + kt * 4, sf + kt * kMxTileBytes);
@@ -531,7 +531,7 @@ mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     // every MMA is complete and every load has been used: the sums go where the ring was
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    if (mbar_wait(tfull, 0, abort_flag, kStatusGemmTimeout) && m_idx * BM + quarter * 32 < args.M) {
+    if (mbar_wait_warp(tfull, 0, abort_flag, kStatusGemmTimeout) && m_idx * BM + quarter * 32 < args.M) {
       tc_fence_after();
       float* dst = reinterpret_cast<float*>(smem) + row * S_PITCH;
 #pragma unroll 1

@@ -556,6 +556,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int idx) -> uint32_t { return bar0 + idx * 8; };
   auto wait = [&](int idx, uint32_t parity) -> bool { return mbar_wait(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
+  auto wait_warp = [&](int idx, uint32_t parity) -> bool { return mbar_wait_warp(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const bool more = args.join == 0;   // a cluster's CTAs do one item
@@ -592,11 +593,11 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const uint32_t tmem_base = *tmem_slot;
   const int item_pos = 2 * args.tile_pos;
 
-  // The item after `fetch` others, or -1.  Called by whole warps in step, by one lane of those that load and issue.
-  auto next_item = [&](int fetch) -> int {
+  // The item after `fetch` others, or -1: for one lane of the warps that load and issue, for whole warps.
+  auto next_item = [&](int fetch, auto wait_for) -> int {
     if (!more) return -1;
     const int slot = fetch & 1;
-    if (!wait(L::NF + slot, fetch >> 1)) return -1;
+    if (!wait_for(L::NF + slot, fetch >> 1)) return -1;
     const int next = read_next(sbase + L::NEXT + slot * 16);
     fence_proxy_async_smem();   // read before the scheduler writes there again
     return next;
@@ -639,7 +640,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           g += span.steps;
           full_items += span.steps > 0;
           if (!ok) break;
-          index = next_item(fetch);
+          index = next_item(fetch, wait);
           if (more) mbar_arrive(bar(L::NE + (fetch & 1)));
         }
       }
@@ -655,7 +656,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         for (int j = 0; ok && j < span.steps; ++j) {
           const int key0 = step_key(span, j);
           const int st = (g + j) & 1;
-          if (!(ok = wait(L::VF + st, (uint32_t)(g + j) >> 1))) break;
+          if (!(ok = wait_warp(L::VF + st, (uint32_t)(g + j) >> 1))) break;
           if (is_mixed(args, span, key0)) {
             if (clean_values(sbase + L::V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
             fence_proxy_async_smem();
@@ -666,7 +667,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         }
         g += span.steps;
         if (!ok) break;
-        index = next_item(fetch);
+        index = next_item(fetch, wait_warp);
         __syncwarp();
         if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
       }
@@ -756,7 +757,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           g += steps;
           ++full_items;
         }
-        index = next_item(fetch);
+        index = next_item(fetch, wait);
         if (more) mbar_arrive(bar(L::NE + (fetch & 1)));
       }
     }
@@ -806,6 +807,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (ok && steps > 0) ok = wait(L::OF + t, full_items);
       // the rows to join take the operands' place: no MMA of the other tile may still read them
       if (ok && args.join && steps > 0) ok = wait(L::OF + (t ^ 1), full_items);
+      ok = __all_sync(0xffffffffu, ok);   // the warp goes on as one
       tc_fence_after();
       const bool parts = args.part_o != nullptr;
       const int64_t out_row = ((int64_t)it.b * args.Sq + min(pos, args.Sq - 1)) * args.H + it.h0 + row_head;
@@ -902,7 +904,7 @@ window_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         __syncwarp();
         cluster_sync_all();   // no CTA retires while another reads its rows
       }
-      index = ok ? next_item(fetch) : -1;
+      index = ok ? next_item(fetch, wait_warp) : -1;
       __syncwarp();
       if (more && lane == 0) mbar_arrive(bar(L::NE + (fetch & 1)));
     }
@@ -939,6 +941,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int idx) -> uint32_t { return bar0 + idx * 8; };
   auto wait = [&](int idx, uint32_t parity) -> bool { return mbar_wait(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
+  auto wait_warp = [&](int idx, uint32_t parity) -> bool { return mbar_wait_warp(bar0 + idx * 8, parity & 1, abort_flag, kStatusFlashTimeout); };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
@@ -1031,7 +1034,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       for (int j = 0; j < steps; ++j) {   // every step, as in window_tile_kernel
         const int key0 = step_key(span, j);
         const int st = j % STAGES;
-        if (!wait(L::VF + st, j / STAGES)) break;
+        if (!wait_warp(L::VF + st, j / STAGES)) break;
         if (is_mixed(args, span, key0)) {
           if (clean_values(sbase + L::V + st * TILE_BYTES, span.n - key0, ft)) *nonfinite = 1;
           fence_proxy_async_smem();
@@ -1116,6 +1119,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     if (ok && uses > 0) ok = wait(L::OF + t, 0);
     // the rows to join take the operands' place: no MMA of the other stream may still read them
     if (ok && args.join && ((steps + t) >> 1) > 0) ok = wait(L::OF + (t ^ 1), 0);
+    ok = __all_sync(0xffffffffu, ok);   // the warp goes on as one
     tc_fence_after();
     const bool parts = args.part_o != nullptr;
     // with nothing to join there is a single step, which is stream 0's
