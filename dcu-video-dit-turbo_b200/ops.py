@@ -55,7 +55,8 @@ class LaunchTimer:
 
     `bound` names the roofline that limits the kernel ("hbm", "int8", "bf16", "mxfp4" or "nvlink") and `work`
     its algorithmic bytes (hbm) or operations per launch, so a caller can turn `ms` into
-    GB/s or TOP/s.  Events are recorded on PyTorch's current stream of the tensor's device
+    GB/s or TOP/s (sizes that lie on the device, a windowed attention's kv_lengths, count as their
+    largest).  Events are recorded on PyTorch's current stream of the tensor's device
     (the stream the kernel is enqueued on); nothing synchronises until `results()`."""
 
     def __init__(self):
@@ -100,7 +101,7 @@ def _call(name: str, t: torch.Tensor, *args, launches: int = 1, work=None) -> No
         _lib.check(st, name)
     if timer is not None:
         e1.record(stream)
-        timer._records.append((name, e0, e1, work))
+        timer._records.append((name, e0, e1, work() if callable(work) else work))
     launch_count += launches
 
 
@@ -809,6 +810,27 @@ def _window_workspace(*sizes: int) -> int:
     return _workspace_of(_lib.current(), *sizes)
 
 
+def _window_work(b: int, h: int, hkv: int, sq: int, sk: int, left: int, right: int, sinks: int) -> tuple[str, int]:
+    """What bounds a windowed attention call whose sequences all have sk keys, and how much of it: the
+    visible pairs' operations, or the bytes of q, out and the keys and values that some query sees
+    where those take longer (a B200 does some 260 operations in the time of a byte)."""
+    p0, p1 = sk - sq, sk - 1                                # the queries' positions
+
+    def total(shift: int, top: int) -> int:
+        """Sum of p + shift within [0, top] over the positions."""
+        low, high = max(p0, -shift), min(p1, top - shift)   # where it is neither limit
+        inside = (low + high + 2 * shift) * (high - low + 1) // 2 if high >= low else 0
+        return inside + top * (p1 - max(p0 - 1, high))
+
+    # the window of p is [clamp(p - left), clamp(p + right + 1)), the first keys before it come on top
+    pairs = (sq * sk if right < 0 else total(right + 1, sk)) - (0 if left < 0 else total(-left, sk) - total(-left, min(sinks, sk)))
+    begin = 0 if left < 0 else max(p0 - left, 0)
+    end = sk if right < 0 else max(min(p1 + right + 1, sk), 0)
+    keys = max(end - begin, 0) + min(sinks, begin)
+    flops, size = 4 * 128 * b * h * pairs, 2 * 128 * b * (2 * h * sq + 2 * hkv * keys)
+    return ("bf16", flops) if flops > 260 * size else ("hbm", size)
+
+
 def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, left: int, right: int,
                     sinks: int = 0, kv_lengths: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 attention forward of q [B,H,Sq,128] over k, v [B,Hkv,Sk,128] (Hkv divides H; any
@@ -852,10 +874,10 @@ def window_fwd_bhsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     storage = torch.empty(b, sq, h, d, dtype=_BF16, device=device)
     need = _window_workspace(b, h, hkv, sq, sk, left, right, sinks)
     workspace = torch.empty(need, dtype=_U8, device=device) if need else None
-    span = sk if left < 0 or right < 0 else min(sk, left + right + 1)
     _call("b2_window_fwd", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), storage.data_ptr(),
           workspace.data_ptr() if need else None, need, lengths, b, h, hkv, sq, sk, qb, qh, qs, kb, kh, ks, vb, vh, vs,
-          scale, left, right, sinks, _stream(q), launches=2 if need else 1, work=("bf16", 4 * b * h * sq * span * d))
+          scale, left, right, sinks, _stream(q), launches=2 if need else 1,
+          work=lambda: _window_work(b, h, hkv, sq, sk, left, right, sinks))
     return storage.transpose(1, 2)
 
 
