@@ -449,6 +449,9 @@ def kernel_row(label, entry, ms, bound, work, pk):
     elif bound == "bf16":
         row.update(unit="TFLOP/s", achieved=work / ms / 1e9, peak=pk["bf16_sustained"],
                    peak_kind=f"dense bf16 sustained, {pk['source']}")
+    elif bound == "mxfp4":
+        row.update(unit="TFLOP/s", achieved=work / ms / 1e9, peak=4 * pk["bf16_burst"],
+                   peak_kind=f"ASSUMED 4 x bf16 burst ({pk['source']}); no measured MXFP4 peak")
     elif bound == "nvlink":
         # bytes this GPU stores into its peers' memory; 770 GB/s is the peer-copy rate per
         # direction measured on this pool's B200s (nominal 900)
