@@ -81,7 +81,9 @@ def grid_positions(tokens: int, height: int = 22, width: int = 38) -> torch.Tens
 class DiTBlock:
     """`window=(left, right)` and `sinks` restrict attention to a sliding window of token positions
     and the first tokens (`ops.window_fwd_bhsd`; None: full attention).  Parameters with MXFP4
-    weights (`make_block_params(weights="mxfp4")`) run the four linears in that format, on one GPU."""
+    weights (`make_block_params(weights="mxfp4")`) run the four linears in that format, on one GPU; their
+    gated residual is a kernel of its own and SwiGLU part of the second projection's quantiser, so
+    the attributes `fuse_residual` and `fuse_swiglu` are then False whatever was asked for."""
 
     def __init__(self, params: dict, sp: UlyssesSP | None = None, head_chunks: int = 1,
                  overlap: bool = True, fuse_residual: bool = True, fuse_swiglu: bool = True,
@@ -93,7 +95,8 @@ class DiTBlock:
         self.mxfp4 = "w4_qkv" in params
         if self.mxfp4 and sp is not None and sp.world > 1:
             raise ValueError("MXFP4 weights run on one GPU: the sequence-parallel ends quantise to int8")
-        self.fuse_residual = fuse_residual   # gated residual in the GEMM epilogue where it pays (same bits either way)
+        # gated residual in the int8 GEMM's epilogue where it pays (same bits either way)
+        self.fuse_residual = bool(fuse_residual) and not self.mxfp4
         # SwiGLU in fc1's epilogue (same bits either way): the [L, 2*ffn] projection never reaches
         # memory; needs fc1's rows interleaved gate/up in groups of 64, prepared once here
         self.fuse_swiglu = bool(fuse_swiglu) and not self.mxfp4 and params["ffn"] % ops.SWIGLU_GROUP == 0
