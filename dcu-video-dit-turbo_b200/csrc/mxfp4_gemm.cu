@@ -422,12 +422,6 @@ constexpr int S_PITCH = SBN + 4;           // floats per row of a CTA's sums: ro
 static_assert(BM * S_PITCH * 4 <= S_SF, "the sums take the place of the operand ring");
 static_assert(S_TOTAL <= SMEM_LIMIT, "shared memory budget");
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 mxfp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                         const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
