@@ -8,9 +8,9 @@
 // Bound by memory: 4 bytes in and 2 + 1 (2 + 17/32) bytes out per element.  A row is held by TPR
 // threads in registers from its only read to its quantised write; y is never rounded to bf16 in
 // between.  A thread keeps the same columns of every row, so the weight is read once per CTA.
-// Measured: int8 109099 x 3072 378 us = 6.2 TB/s, 23638 x 3072 88 us = 5.8; MXFP4 361 and 85 us.
+// Measured: int8 109099 x 3072 376 us = 6.2 TB/s, 23638 x 3072 88 us = 5.8; MXFP4 360 and 84 us.
 // Roundings: the mean, 1 / sqrt, max|y| / 127 and y / scale are each rounded once, to the nearest fp32
-// (0 to 3 % more time than products with rounded reciprocals and the fast 1 / sqrt, 5 % at 16384 columns).
+// (0 to 3 % more time than products with rounded reciprocals and the fast 1 / sqrt, int8 at 16384 columns 4 %).
 // The elements divide by the fp32 scale that is stored, so q * scale is within half a step of y.
 #include "b2_common.cuh"
 #include "b2_launch.h"
@@ -21,6 +21,12 @@ namespace {
 
 constexpr int kThreads = 256;   // of the generic kernel
 
+// 1 / n as a sum of two fp32
+struct Reciprocal {
+  float high, low;
+  __host__ __device__ constexpr explicit Reciprocal(double n) : high((float)(1.0 / n)), low((float)(1.0 / n - (double)(float)(1.0 / n))) {}
+};
+
 struct RmsArgs {
   const uint4* x;
   const uint4* residual;   // null: s = x and nothing is stored to `sum`
@@ -30,15 +36,16 @@ struct RmsArgs {
   void* scale;             // fp32 [M] or scale tiles
   int64_t M;
   int cvec;                // C / 8
-  double inv_c;            // 1 / C
+  Reciprocal inv_c{1.0};   // of C
   float eps;
 };
 
-// v / n rounded to the nearest fp32, inv_n = 1 / n in 64 bits: a quotient of two 24-bit numbers is no
-// nearer to the middle between two fp32 than 2^-49 of itself, and the product is within 2^-52.
-__device__ __forceinline__ float quotient(float v, double inv_n) { return (float)((double)v * inv_n); }
+// v / n, rounded once (from within 2^-48 of itself); infinities and NaN as they are
+__device__ __forceinline__ float quotient(float v, const Reciprocal& inv) {
+  return fabsf(v) <= 3.4028234e38f ? fmaf(v, inv.high, v * inv.low) : v;
+}
 // 1 / sqrt(sum of squares / C + eps)
-__device__ __forceinline__ float row_rstd(float ss, double inv_c, float eps) {
+__device__ __forceinline__ float row_rstd(float ss, const Reciprocal& inv_c, float eps) {
   return __frsqrt_rn(__fadd_rn(quotient(ss, inv_c), eps));
 }
 // A row's int8 scale, from its largest magnitude, and 1 / scale as a sum of two fp32.  Rows with a NaN or an
@@ -47,7 +54,7 @@ struct Int8Scale {
   float s, inv, inv_low;
   bool zero_row;
   __device__ __forceinline__ explicit Int8Scale(float absmax) {
-    s = absmax != absmax ? absmax : fmaxf(quotient(absmax, 1.0 / 127.0), 1.0e-30f);
+    s = absmax != absmax ? absmax : fmaxf(quotient(absmax, Reciprocal(127.0)), 1.0e-30f);
     zero_row = !(s <= 3.4028234e38f);
     inv = __frcp_rn(s);
     inv_low = fmaf(-s, inv, 1.0f) * inv;
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(kThreads)
 rmsnorm_residual_quant_generic_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ residual,
                                       const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ sum,
                                       int8_t* __restrict__ q, float* __restrict__ scale, int64_t M, int64_t C,
-                                      double inv_c, float eps) {
+                                      Reciprocal inv_c, float eps) {
   __shared__ float red[2][kThreads / 32];
   for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
     const int64_t at = row * C;
@@ -354,7 +361,7 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
     const int64_t cap = (int64_t)kNumSMsB200 * 8;
     rmsnorm_residual_quant_generic_kernel<<<(unsigned)(M < cap ? M : cap), kThreads, 0, stream>>>(
         (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)weight, (__nv_bfloat16*)sum,
-        (int8_t*)q, (float*)scale, M, C, 1.0 / (double)C, eps);
+        (int8_t*)q, (float*)scale, M, C, Reciprocal((double)C), eps);
     return check_launch("rmsnorm_residual_quant");
   }
   RmsArgs a;
@@ -366,7 +373,7 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
   a.scale = scale;
   a.M = M;
   a.cvec = (int)(C / 8);
-  a.inv_c = 1.0 / (double)C;
+  a.inv_c = Reciprocal((double)C);
   a.eps = eps;
   if (!vector) {
 #define B2_RMS_ODD(THREADS, TPR, VPT)                                                                            \

@@ -87,3 +87,27 @@ def test_every_step_is_rounded_once(cuda_pkg, c, eps):
         code, byte = R.mx_quantize(y.double())
         q, s, _ = (t.cpu() for t in cuda_pkg.ops.rmsnorm_residual_mxfp4(xd, None, wd, eps))
         assert torch.equal(s, R.mx_tiles(byte)) and torch.equal(R.mx_codes(q) & 7, code & 7)
+
+
+@pytest.mark.parametrize("c", [32, 37, 127, 128, 1001, 4096])
+def test_sums_and_products_past_the_range(cuda_pkg, c):
+    """A sum of squares past fp32's range is an infinity, whose row is zeros; a product past it is one, which
+    the scale keeps."""
+    ops = cuda_pkg.ops
+    x = torch.randn((4, c), generator=torch.Generator().manual_seed(c)).to(torch.bfloat16)
+    x[0], x[2] = 3e19, -3e38
+    w = torch.ones(c, dtype=torch.bfloat16)
+    q, s, _ = (t.cpu() for t in ops.rmsnorm_residual_quant(x.to(DEV), None, w.to(DEV)))
+    assert not q[0].any() and not q[2].any() and (s[[0, 2]] == torch.tensor(1e-30)).all()
+    assert torch.isfinite(s).all() and q[1].any() and q[3].any()
+    x[1], x[3] = 1.0, 1.0
+    x[1, 1] = 4.0                                           # the row's largest, and more than the others' mean
+    w[1] = 3e38
+    want = rounded_norm(x[1::2].double(), w, 1e-6)
+    q, s, _ = (t.cpu() for t in ops.rmsnorm_residual_quant(x.to(DEV), None, w.to(DEV)))
+    for i, row in ((1, 0), (3, 1)):
+        if torch.isfinite(want[row]).all():
+            assert torch.isfinite(s[i]).all() and q[i].any()
+        else:
+            assert torch.isinf(s[i]).all() and not q[i].any()
+    assert not torch.isfinite(want[0]).all() and torch.isfinite(want[1]).all()
