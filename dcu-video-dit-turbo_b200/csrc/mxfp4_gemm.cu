@@ -16,7 +16,7 @@
 // 128 x 256 tile of one CTA): at 4 bits the tensor core eats a stage in 512 clocks, and what an SM
 // can draw from L2 in that time is what bounds the product.  The leader issues for both; W's scales
 // are needed whole in both tensor memories.  TMA loads are plain per-CTA ones.
-// Measured, 23638 x 9216 x 3072: 263 us, 5.09 PFLOP/s (18944 x 2048 x 8192: 107 us, 5.96 PFLOP/s); the
+// Measured, 23638 x 9216 x 3072: 266 us, 5.03 PFLOP/s (18944 x 2048 x 8192: 107 us, 5.96 PFLOP/s); the
 // loads alone take 221 us and the MMAs alone 217.  One CTA per tile took 458 us, pairs 403; the rest was
 // the issuing warp: with a lane-divergent region around the MMAs and a second commit per stage a stage
 // took 1260 clocks, with the whole warp in step and one commit 730.
