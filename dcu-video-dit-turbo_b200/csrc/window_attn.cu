@@ -36,10 +36,10 @@
 //
 // Bound by the tensor cores (4 * 128 FLOP per visible pair and head) when many rows share the keys,
 // by reading K and V once for single tokens.  Measured: 24 heads x 23638, window 3344 each way, 836 first
-// keys 1.82 to 1.93 ms over five boxes, 1.10 PFLOP/s over the visible pairs at 1.83; a step of 256 rows x
+// keys 1.82 to 1.93 ms over five GPUs, 1.10 PFLOP/s over the visible pairs at 1.83; a step of 256 rows x
 // 128 keys takes 1.77 us, of which the tensor cores work 1.1: a tile's chain scores -> maximum ->
 // exponentials -> P -> product -> next scores is what it waits for.  24 heads x 8192, window 511: 92 to 116
-// us over the boxes, a fifth of it the items' output.
+// us over these, a fifth of it the items' output.
 // 8 x 6 key heads, single tokens, 4224 keys each: 104 MB in 25 us, of which 8 are set-up, first loads and
 // the join.
 #include "flash_common.cuh"
